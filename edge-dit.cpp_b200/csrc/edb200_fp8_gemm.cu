@@ -1,0 +1,479 @@
+// Matrix product over e4m3 operands with one f32 scale for each block of 128 k (edb200_mul_mat_fp8):
+//
+//   y[m, n] = sum_b  xs[m, b] ws[n / 128, b]  sum_{k in block b} x[m, k] w[n, k]        (+ bias, activation, ...)
+//
+// The inner sums run on the tensor cores (tcgen05 kind::f8f6f4, f32 accumulators in tensor memory).  A block's scale
+// differs from row to row, so its sum cannot stay in one accumulator over all of k: the accumulators alternate between
+// two places in tensor memory, one written by block b + 1's four MMAs while eight warps read the other, multiply by the
+// block's scale and add into f32 registers ("promotion").  With tokens in the 128 lanes of tensor memory and features in
+// its columns, xs[m, b] ws[n / 128, b] is one number per thread and the promotion one FMA per element.
+//
+// A 128 x 128-byte operand tile is exactly one block of 128 e4m3 values per row: one TMA box with 128-byte swizzle, four
+// MMAs of 32 k.  Rows beyond m and n and values beyond k are zero-filled by TMA and masked in the epilogue.
+#include "edb200_internal.h"
+#include "edb200_ptx.cuh"
+#include "edb200_fp8.cuh"
+
+#include <cstring>
+
+namespace edb {
+namespace f8g {
+
+constexpr int BK = 128;                       // bytes = values of a k block
+constexpr uint32_t kFmtE4M3 = 0;              // kind::f8f6f4
+constexpr int PITCH = 36;                     // words between rows of an epilogue staging buffer (32 + 4: no conflicts)
+
+struct Params {
+    const float* xs;
+    const float* ws;
+    long long ld_xs, ld_ws;
+    const float* bias;
+    const float* residual;
+    const float* gate;
+    void* out;
+    float* out_scale;
+    long long ldo, ld_res, ld_os;
+    int M, N, kblocks;
+    int act, out_dtype;
+    int m_tiles;
+    int* err;
+};
+
+__device__ __forceinline__ void mma_f8_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// acc[i] += s * r[i], two elements an instruction.
+template <int N>
+__device__ __forceinline__ void promote(float (&acc)[N], int at, const uint32_t (&r)[32], float s) {
+    uint64_t ss;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(ss) : "f"(s));
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        uint64_t a, b;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(acc[at + i]), "f"(acc[at + i + 1]));
+        asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "r"(r[i]), "r"(r[i + 1]));
+        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(b), "l"(ss));
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[at + i]), "=f"(acc[at + i + 1]) : "l"(a));
+    }
+}
+
+// The activations by exp and one division: gelu_tanh(v) = v / (1 + exp(-2 u)), exact to a few f32 roundings.
+__device__ __forceinline__ float act_one(float v, int act) {
+    if (act == EDB200_ACT_GELU_TANH) {
+        const float u = 0.7978845608028654f * v * fmaf(0.044715f * v, v, 1.0f);
+        return __fdividef(v, 1.0f + __expf(-2.0f * u));
+    }
+    if (act == EDB200_ACT_SILU) return __fdividef(v, 1.0f + __expf(-v));
+    return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));   // EDB200_ACT_GELU_ERF
+}
+template <int N>
+__device__ __forceinline__ void bias_act(float (&v)[N], const float* bias, int act) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(bias + i);
+        v[i] += b.x, v[i + 1] += b.y, v[i + 2] += b.z, v[i + 3] += b.w;
+    }
+    if (act != EDB200_ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = act_one(v[i], act);
+    }
+}
+
+// A warp's staged rows [32][32 words] to memory, `words` (16 or 32) of each row, 16 bytes a lane: whole 64- or 128-byte
+// runs of a row per store.  row0 / byte0: first row and first byte in a row of the staged piece; row_bytes: end of a row.
+template <typename F>
+__device__ __forceinline__ void copy_out(const float* stage, int words, int lane, const F& put) {
+    const int per = words / 4;               // lanes a row: 8 or 4
+    const int r0 = lane / per, c = (lane - r0 * per) * 4;
+    for (int r = r0; r < 32; r += 32 / per) put(r, c, *reinterpret_cast<const uint4*>(stage + r * PITCH + c));
+}
+
+// Epilogue of one thread's row m, columns n0 .. n0 + N - 1 (already biased and activated, in registers), through the
+// warp's staging buffer.  amax: of the row's 128 columns (e4m3 output).
+template <int N>
+__device__ __forceinline__ void store_rows(const Params& P, const float (&v)[N], int m_first, int n0, int lane, float* stage,
+                                           const float* gate, float amax) {
+    const bool inside = n0 + N <= P.N;
+    if (P.out_dtype == EDB200_TYPE_F32) {
+#pragma unroll
+        for (int c = 0; c < N / 32; ++c) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                *reinterpret_cast<float4*>(stage + lane * PITCH + i) = make_float4(v[32 * c + i], v[32 * c + i + 1], v[32 * c + i + 2], v[32 * c + i + 3]);
+            }
+            __syncwarp();
+            copy_out(stage, 32, lane, [&](int r, int col, uint4 u) {
+                const long long m = m_first + r;
+                const int n = n0 + 32 * c + col;
+                if (m >= P.M || n >= P.N) return;
+                float4 x = *reinterpret_cast<float4*>(&u);
+                float* o = static_cast<float*>(P.out) + m * P.ldo + n;
+                if (inside || n + 4 <= P.N) {
+                    if (P.gate != nullptr) {
+                        const float4 g = *reinterpret_cast<const float4*>(gate + 32 * c + col);
+                        const float4 q = *reinterpret_cast<const float4*>(P.residual + m * P.ld_res + n);
+                        x = make_float4(fmaf(g.x, x.x, q.x), fmaf(g.y, x.y, q.y), fmaf(g.z, x.z, q.z), fmaf(g.w, x.w, q.w));
+                    }
+                    *reinterpret_cast<float4*>(o) = x;
+                } else {
+                    const float w[4] = {x.x, x.y, x.z, x.w};
+                    for (int e = 0; e < P.N - n; ++e) {
+                        float y = e == 0 ? w[0] : e == 1 ? w[1] : w[2];
+                        if (P.gate != nullptr) y = fmaf(gate[32 * c + col + e], y, P.residual[m * P.ld_res + n + e]);
+                        o[e] = y;
+                    }
+                }
+            });
+        }
+    } else if (P.out_dtype != EDB200_TYPE_F8_E4M3) {
+        const bool bf = P.out_dtype == EDB200_TYPE_BF16;
+#pragma unroll
+        for (int c = 0; c < N / 64; ++c) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 64; i += 8) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float a = v[64 * c + i + 2 * j], b = v[64 * c + i + 2 * j + 1];
+                    if (bf) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+                        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                    } else {
+                        const __half2 h = __floats2half2_rn(a, b);
+                        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                }
+                *reinterpret_cast<uint4*>(stage + lane * PITCH + i / 2) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            __syncwarp();
+            copy_out(stage, 32, lane, [&](int r, int col, uint4 u) {
+                const long long m = m_first + r;
+                const int n = n0 + 64 * c + 2 * col;
+                if (m >= P.M || n >= P.N) return;
+                uint16_t* o = static_cast<uint16_t*>(P.out) + m * P.ldo + n;
+                if (inside || n + 8 <= P.N) {
+                    *reinterpret_cast<uint4*>(o) = u;
+                } else {
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (n + e < P.N) o[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+                    }
+                }
+            });
+        }
+    } else {
+        float s, inv;
+        f8_scale(amax, s, inv);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < N; i += 16) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = f8_pack4(f8_scaled(v[i + 4 * j], inv), f8_scaled(v[i + 4 * j + 1], inv), f8_scaled(v[i + 4 * j + 2], inv),
+                                f8_scaled(v[i + 4 * j + 3], inv));
+            }
+            *reinterpret_cast<uint4*>(stage + lane * PITCH + i / 4) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (m_first + lane < P.M && (n0 & 127) == 0 && n0 < P.N) {
+            P.out_scale[static_cast<long long>(m_first + lane) * P.ld_os + (n0 >> 7)] = s;
+        }
+        __syncwarp();
+        copy_out(stage, N / 4, lane, [&](int r, int col, uint4 u) {
+            const long long m = m_first + r;
+            const int n = n0 + 4 * col;
+            if (m >= P.M || n >= P.N) return;
+            uint8_t* o = static_cast<uint8_t*>(P.out) + m * P.ldo + n;
+            if (inside || n + 16 <= P.N) {
+                *reinterpret_cast<uint4*>(o) = u;
+            } else {
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    if (n + e < P.N) o[e] = static_cast<uint8_t>(w[e >> 2] >> (8 * (e & 3)));
+                }
+            }
+        });
+    }
+}
+
+// Largest magnitude of a thread's columns n0 .. that lie inside N.
+template <int N>
+__device__ __forceinline__ float row_magnitude(const float (&v)[N], int n0, int n_end) {
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) a = fmaxf(a, n0 + i < n_end ? f8_magnitude(v[i]) : 0.0f);
+    return a;
+}
+
+// ------------------------------------------------------------------ one CTA per 128 tokens x 128 features
+namespace tile {
+constexpr int STAGES = 5;
+constexpr int A_BYTES = 128 * BK, STAGE_BYTES = 2 * A_BYTES;
+constexpr int WARPS = 8;                                        // promotion warps
+constexpr int CPT = 64;                                         // columns of a promotion thread
+constexpr int OFF_STAGE = STAGES * STAGE_BYTES;
+constexpr int OFF_VEC = OFF_STAGE + WARPS * 32 * PITCH * 4;     // bias [128], gate [128], row maxima [2][128]
+constexpr int OFF_BAR = OFF_VEC + 512 * 4;
+constexpr int SMEM_BYTES = OFF_BAR + 256 + 1024;
+constexpr int THREADS = 32 * (WARPS + 2);
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory plan");
+}  // namespace tile
+
+__global__ void __launch_bounds__(tile::THREADS, 1)
+fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                const __grid_constant__ Params P) {
+    using namespace tile;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* s_bias = reinterpret_cast<float*>(smem + OFF_VEC);
+    float* s_gate = s_bias + 128;
+    float* s_max = s_gate + 128;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + OFF_BAR);   // [STAGES]
+    uint64_t* empty = full + STAGES;                                // [STAGES]
+    uint64_t* acc_full = empty + STAGES;                            // [2]
+    uint64_t* acc_empty = acc_full + 2;                             // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n_tile = blockIdx.x / P.m_tiles, m_tile = blockIdx.x - n_tile * P.m_tiles;
+    const int n0 = n_tile * 128, m0 = m_tile * 128;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], WARPS);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 256);
+        tmem_relinquish();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&map_x);
+        tma_prefetch_desc(&map_w);
+    }
+    if (warp >= 2) {
+        const int t = threadIdx.x - 64, n = n0 + (t & 127);
+        const float* src = t < 128 ? P.bias : P.gate;
+        s_bias[t] = (src != nullptr && n < P.N) ? __ldg(src + n) : 0.0f;   // s_gate follows s_bias
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        uint32_t s = 0, ph = 0;
+        for (int b = 0; b < P.kblocks; ++b) {
+            if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, P.err)) break;
+            if (elect_one()) {
+                uint8_t* stage = smem + s * STAGE_BYTES;
+                mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
+                tma_load_2d(stage, &map_x, &full[s], b * BK, m0);
+                tma_load_2d(stage + A_BYTES, &map_w, &full[s], b * BK, n0);
+            }
+            __syncwarp();
+            if (++s == STAGES) {
+                s = 0;
+                ph ^= 1u;
+            }
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc = make_idesc(kDFmtF32, kFmtE4M3, kFmtE4M3, 0, 0, 128, 128);
+        uint32_t s = 0, ph = 0;
+        for (int b = 0; b < P.kblocks; ++b) {
+            const uint32_t buf = b & 1, aph = (b >> 1) & 1;
+            if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag, P.err)) break;
+            if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
+            tc_fence_after_sync();
+            if (elect_one()) {
+                const uint32_t a_addr = smem_u32(smem + s * STAGE_BYTES), b_addr = a_addr + A_BYTES;
+#pragma unroll
+                for (int j = 0; j < BK / 32; ++j) {
+                    mma_f8_ss(tmem_base + buf * 128, make_smem_desc_sw128(a_addr + j * 32, 16, 1024),
+                              make_smem_desc_sw128(b_addr + j * 32, 16, 1024), idesc, j > 0 ? 1u : 0u);
+                }
+                mma_commit(&empty[s]);
+                mma_commit(&acc_full[buf]);
+            }
+            __syncwarp();
+            if (++s == STAGES) {
+                s = 0;
+                ph ^= 1u;
+            }
+        }
+    } else {
+        const int quarter = warp & 3, side = (warp - 2) >> 2;   // lanes of tensor memory, half of the columns
+        const int row = quarter * 32 + lane;
+        const int m = m0 + row < P.M ? m0 + row : P.M - 1;      // rows past the end follow the last one, store nothing
+        const float* xs = P.xs + m * P.ld_xs;
+        const float* ws = P.ws + n_tile * P.ld_ws;
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + side * CPT;
+        float acc[CPT];
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) acc[i] = 0.0f;
+        float scale = __ldg(xs) * __ldg(ws);
+        bool ok = true;
+        for (int b = 0; b < P.kblocks; ++b) {
+            const uint32_t buf = b & 1, aph = (b >> 1) & 1;
+            const int nb = b + 1 < P.kblocks ? b + 1 : b;
+            const float next = __ldg(xs + nb) * __ldg(ws + nb);
+            ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aph, abort_flag, P.err));
+            if (!ok) break;
+            tc_fence_after_sync();
+            uint32_t r0[32], r1[32];
+            tmem_ld_32x32b_x32(taddr + buf * 128, r0);
+            tmem_ld_32x32b_x32(taddr + buf * 128 + 32, r1);
+            tmem_wait_ld();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            promote(acc, 0, r0, scale);
+            promote(acc, 32, r1, scale);
+            scale = next;
+        }
+        const int nc = n0 + side * CPT;
+        float amax = 0.0f;
+        if (ok) bias_act(acc, s_bias + side * CPT, P.act);
+        if (P.out_dtype == EDB200_TYPE_F8_E4M3) {   // uniform: the row's other half lies in the other warp group
+            s_max[side * 128 + row] = row_magnitude(acc, nc, P.N);
+            named_bar_sync(1, 32 * WARPS);
+            amax = fmaxf(s_max[row], s_max[128 + row]);
+        }
+        if (ok) store_rows(P, acc, m0 + quarter * 32, nc, lane, reinterpret_cast<float*>(smem + OFF_STAGE) + (warp - 2) * 32 * PITCH, s_gate + side * CPT, amax);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (*abort_flag) {
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);   // let copies and MMAs in flight land
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, 256);
+    }
+}
+
+// Sets a kernel's dynamic shared memory once per device.
+template <typename K>
+static edb200_status_t allow_smem(K kern, int bytes, bool (&done)[64]) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (done[dev]) return EDB200_OK;
+    EDB_TRY(check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute(mul_mat_fp8)"));
+    done[dev] = true;
+    return EDB200_OK;
+}
+
+// Operand rows of k bytes as boxes of 128 bytes x box_rows (a single row's pitch may be anything).
+static edb200_status_t operand_map(CUtensorMap* map, const void* base, int64_t k, int64_t rows, int64_t ld, uint32_t box_rows) {
+    const uint64_t pitch = rows > 1 ? (uint64_t)ld : ((uint64_t)k + 15) / 16 * 16;
+    return make_tmap_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, (uint64_t)k, (uint64_t)rows, pitch, BK, box_rows,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+static edb200_status_t launch_tile(const edb200_fp8_weight_t& w, const void* x, int64_t m, int64_t ldx, Params& P, cudaStream_t s) {
+    CUtensorMap map_x, map_w;
+    EDB_TRY(operand_map(&map_x, x, w.k, m, ldx, 128));
+    EDB_TRY(operand_map(&map_w, w.w, w.k, w.n, w.ldw, 128));
+    static bool done[64] = {false};
+    EDB_TRY(allow_smem(fp8_tile_kernel, tile::SMEM_BYTES, done));
+    P.m_tiles = static_cast<int>((m + 127) / 128);
+    const int64_t tiles = (int64_t)P.m_tiles * ((w.n + 127) / 128);
+    if (tiles > 0x7fffffff) return fail(EDB200_ERR_UNSUPPORTED, "mul_mat_fp8: too many output tiles");
+    fp8_tile_kernel<<<static_cast<unsigned>(tiles), tile::THREADS, tile::SMEM_BYTES, s>>>(map_x, map_w, P);
+    count_launch();
+    return check_cuda(cudaGetLastError(), "mul_mat_fp8 launch");
+}
+
+}  // namespace f8g
+}  // namespace edb
+
+extern "C" edb200_status_t edb200_mul_mat_fp8(const edb200_fp8_weight_t* w, const void* x, const float* x_scale, int64_t m,
+                                              int64_t ldx, int64_t ld_xs, const edb200_epilogue_t* ep, float* out_scale,
+                                              int64_t ld_out_scale, void* stream) {
+    using namespace edb;
+    if (w == nullptr || ep == nullptr) return fail(EDB200_ERR_INVALID, "mul_mat_fp8: null argument");
+    const int64_t big = 0x7fffff00ll;
+    if (m < 0 || m > big || w->n < 1 || w->n > big || w->k < 1 || w->k > big) {
+        return fail(EDB200_ERR_INVALID, "mul_mat_fp8: m >= 0, n >= 1 and k >= 1, each below 2^31 - 256");
+    }
+    if (ep->split_n != 0 || ep->pack != nullptr || ep->split_k != EDB200_SPLIT_K_NEVER) {
+        return fail(EDB200_ERR_UNSUPPORTED, "mul_mat_fp8: split_n, split_k and pack belong to mul_mat_q");
+    }
+    if (ep->act < EDB200_ACT_NONE || ep->act > EDB200_ACT_GELU_ERF) return fail(EDB200_ERR_INVALID, "mul_mat_fp8: bad act");
+    const int dt = ep->out_dtype;
+    const bool f8 = dt == EDB200_TYPE_F8_E4M3;
+    if (dt != EDB200_TYPE_F32 && dt != EDB200_TYPE_F16 && dt != EDB200_TYPE_BF16 && !f8) {
+        return fail(EDB200_ERR_INVALID, "mul_mat_fp8: out_dtype must be f32, f16, bf16 or e4m3");
+    }
+    if (m == 0) return EDB200_OK;
+    if (w->w == nullptr || w->scale == nullptr || x == nullptr || x_scale == nullptr || ep->out == nullptr) {
+        return fail(EDB200_ERR_INVALID, "mul_mat_fp8: null argument");
+    }
+    const int64_t kb = (w->k + 127) / 128, nb = (w->n + 127) / 128;
+    auto at = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
+    // a single row's stride is not used
+    if ((m > 1 && (ldx < w->k || ldx % 16)) || (at(x) & 15u) || (w->n > 1 && (w->ldw < w->k || w->ldw % 16)) || (at(w->w) & 15u)) {
+        return fail(EDB200_ERR_INVALID, "mul_mat_fp8: rows of x and w must be 16-byte aligned and hold k values");
+    }
+    if ((m > 1 && ld_xs < kb) || (nb > 1 && w->ld_scale < kb) || ((at(x_scale) | at(w->scale)) & 3u)) {
+        return fail(EDB200_ERR_INVALID, "mul_mat_fp8: scale rows must be 4-byte aligned and hold ceil(k / 128) values");
+    }
+    const int esz = dt == EDB200_TYPE_F32 ? 4 : f8 ? 1 : 2;
+    if ((m > 1 && (ep->ldo < w->n || (ep->ldo * esz) % 16)) || (at(ep->out) & 15u)) {
+        return fail(EDB200_ERR_INVALID, "mul_mat_fp8: out rows must be 16-byte aligned and ldo >= n");
+    }
+    if ((at(ep->bias) | at(ep->gate)) & 3u) return fail(EDB200_ERR_INVALID, "mul_mat_fp8: bias and gate must be 4-byte aligned");
+    if (ep->gate != nullptr && (dt != EDB200_TYPE_F32 || ep->residual == nullptr || (m > 1 && (ep->ld_res < w->n || ep->ld_res % 4)) ||
+                                (at(ep->residual) & 15u))) {
+        return fail(EDB200_ERR_INVALID, "mul_mat_fp8: gated residual needs f32 out and residual rows of n values, 16-byte aligned");
+    }
+    if (f8 != (out_scale != nullptr) || (f8 && ((m > 1 && ld_out_scale < nb) || (at(out_scale) & 3u)))) {
+        return fail(EDB200_ERR_INVALID, "mul_mat_fp8: e4m3 out, and only it, needs out_scale with ceil(n / 128) columns");
+    }
+    int* err = device_error_word();
+    if (err == nullptr) return fail(EDB200_ERR_CUDA, "mul_mat_fp8: no CUDA device");
+    f8g::Params P;
+    memset(&P, 0, sizeof(P));
+    P.xs = x_scale;
+    P.ws = w->scale;
+    P.ld_xs = ld_xs;
+    P.ld_ws = w->ld_scale;
+    P.bias = ep->bias;
+    P.residual = ep->residual;
+    P.gate = ep->gate;
+    P.out = ep->out;
+    P.out_scale = out_scale;
+    P.ldo = ep->ldo;
+    P.ld_res = ep->ld_res;
+    P.ld_os = ld_out_scale;
+    P.M = static_cast<int>(m);
+    P.N = static_cast<int>(w->n);
+    P.kblocks = static_cast<int>(kb);
+    P.act = ep->act;
+    P.out_dtype = dt;
+    P.err = err;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    ProfScope prof(s, PROF_GEMM, 2.0 * (double)m * (double)w->n * (double)w->k,
+                   (double)w->n * (double)w->k + (double)m * (double)w->k + (double)m * (double)w->n * esz);
+    return f8g::launch_tile(*w, x, m, ldx, P, s);
+}

@@ -1,0 +1,183 @@
+// Quantisation to e4m3 with one f32 scale for each block of 1 x 128 or 128 x 128 values.
+//
+//   a = max(max finite |x|, 2^-100),   scale = a / 448,   q = e4m3(x * (448 / a))
+//
+// Bound: HBM.  Each value is read once, kept in registers across the block's maximum, and written as a byte.
+// Eight lanes own one row's 128 columns: lane l takes columns 64 j + 8 l .. + 7 (j = 0, 1), so a warp's load of
+// 16-bit values is four full 128-byte lines and the block maximum is three shuffles.
+#include "edb200_internal.h"
+#include "edb200_fp8.cuh"
+
+namespace edb {
+namespace f8q {
+
+constexpr int THREADS = 256;
+
+// The 16 values lane l of a group holds of one row's block: columns c0 + 64 j + 8 l + e.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load16(const T* row, int c0, int l, int k, bool live, float (&v)[16]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int c = c0 + 64 * j + 8 * l;
+        float w[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (VEC && live && c + 8 <= k) {
+            load8(row + c, w);
+        } else if (live) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (c + e < k) w[e] = widen<T>(row[c + e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * j + e] = w[e];
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store16(uint8_t* row, int c0, int l, int k, const float (&v)[16], float inv) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int c = c0 + 64 * j + 8 * l;
+        if (c >= k) continue;
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = f8_scaled(v[8 * j + e], inv);
+        const uint32_t lo = f8_pack4(w[0], w[1], w[2], w[3]), hi = f8_pack4(w[4], w[5], w[6], w[7]);
+        if (VEC && c + 8 <= k) {
+            *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (c + e < k) row[c + e] = static_cast<uint8_t>((e < 4 ? lo : hi) >> (8 * (e & 3)));
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ float magnitude16(const float (&v)[16]) {
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) a = fmaxf(a, f8_magnitude(v[i]));
+    return a;
+}
+
+// 1 x 128: a group of eight lanes per block; I is the index type that holds rows * blocks.
+template <typename T, bool VEC, typename I>
+__global__ void __launch_bounds__(THREADS)
+quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int k, int kb, uint8_t* __restrict__ q, int64_t ldq,
+                     float* __restrict__ scale, int64_t ld_scale) {
+    const int l = threadIdx.x & 7;
+    const I g = static_cast<I>(blockIdx.x) * (THREADS / 8) + (threadIdx.x >> 3);
+    const I row = g / static_cast<I>(kb);
+    const int b = static_cast<int>(g - row * static_cast<I>(kb));
+    const bool live = static_cast<int64_t>(row) < rows;
+    float v[16];
+    load16<T, VEC>(x + static_cast<int64_t>(row) * ldx, b * 128, l, k, live, v);
+    float a = magnitude16(v);
+#pragma unroll
+    for (int m = 4; m > 0; m >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, m));
+    if (!live) return;
+    float s, inv;
+    f8_scale(a, s, inv);
+    store16<VEC>(q + static_cast<int64_t>(row) * ldq, b * 128, l, k, v, inv);
+    if (l == 0) scale[static_cast<int64_t>(row) * ld_scale + b] = s;
+}
+
+// 128 x 128: a CTA per block, 32 rows at a time, all 64 values of a thread in registers.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(THREADS)
+quantize_tiles_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int k, uint8_t* __restrict__ q, int64_t ldq,
+                      float* __restrict__ scale, int64_t ld_scale) {
+    __shared__ float sh[THREADS / 32];
+    const int l = threadIdx.x & 7;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.y) * 128 + (threadIdx.x >> 3);
+    const int c0 = blockIdx.x * 128;
+    float v[4][16];
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t row = row0 + 32 * i;
+        load16<T, VEC>(x + row * ldx, c0, l, k, row < rows, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a = fmaxf(a, magnitude16(v[i]));
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, m));
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) a = fmaxf(a, sh[i]);
+    float s, inv;
+    f8_scale(a, s, inv);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t row = row0 + 32 * i;
+        if (row < rows) store16<VEC>(q + row * ldq, c0, l, k, v[i], inv);
+    }
+    if (threadIdx.x == 0) scale[static_cast<int64_t>(blockIdx.y) * ld_scale + blockIdx.x] = s;
+}
+
+template <typename T>
+static edb200_status_t launch(const T* x, int64_t ldx, int64_t rows, int64_t k, int block_rows, uint8_t* q, int64_t ldq,
+                              float* scale, int64_t ld_scale, cudaStream_t s) {
+    const int64_t kb = (k + 127) / 128;
+    // wide accesses: 16-byte loads of 8 values (two for f32), 8-byte stores
+    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (rows == 1 || (ldx * sizeof(T)) % 16 == 0) &&
+                     (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && (rows == 1 || ldq % 8 == 0);
+    const int ki = static_cast<int>(k);
+    if (block_rows == 1) {
+        const int64_t groups = rows * kb;
+        const int64_t ctas = (groups + THREADS / 8 - 1) / (THREADS / 8);
+        if (ctas > 0x7fffffff) return fail(EDB200_ERR_UNSUPPORTED, "quantize_fp8: more than 2^36 blocks");
+        const unsigned grid = static_cast<unsigned>(ctas);
+        // 32-bit block indices where they hold every block of the grid: one division less in 64 bits per thread
+        if (groups < 0x7fffff00ll) {
+            if (vec) {
+                quantize_rows_kernel<T, true, uint32_t><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, (int)kb, q, ldq, scale, ld_scale);
+            } else {
+                quantize_rows_kernel<T, false, uint32_t><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, (int)kb, q, ldq, scale, ld_scale);
+            }
+        } else {
+            quantize_rows_kernel<T, false, uint64_t><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, (int)kb, q, ldq, scale, ld_scale);
+        }
+    } else {
+        const int64_t rb = (rows + 127) / 128;
+        if (rb > 65535) return fail(EDB200_ERR_UNSUPPORTED, "quantize_fp8: more than 65535 x 128 rows of 128 x 128 blocks");
+        const dim3 grid(static_cast<unsigned>(kb), static_cast<unsigned>(rb));
+        if (vec) {
+            quantize_tiles_kernel<T, true><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, q, ldq, scale, ld_scale);
+        } else {
+            quantize_tiles_kernel<T, false><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, q, ldq, scale, ld_scale);
+        }
+    }
+    count_launch();
+    return check_cuda(cudaGetLastError(), "quantize_fp8 launch");
+}
+
+}  // namespace f8q
+}  // namespace edb
+
+extern "C" edb200_status_t edb200_quantize_fp8(const void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t k, int block_rows,
+                                               void* q, int64_t ldq, float* scale, int64_t ld_scale, void* stream) {
+    using namespace edb;
+    if (x_dtype != EDB200_TYPE_F32 && x_dtype != EDB200_TYPE_F16 && x_dtype != EDB200_TYPE_BF16) {
+        return fail(EDB200_ERR_INVALID, "quantize_fp8: x_dtype must be f32, f16 or bf16");
+    }
+    if (block_rows != 1 && block_rows != 128) return fail(EDB200_ERR_INVALID, "quantize_fp8: block_rows must be 1 or 128");
+    if (rows < 0 || k < 1 || k > 0x7fffff00ll) return fail(EDB200_ERR_INVALID, "quantize_fp8: rows >= 0 and 1 <= k < 2^31 - 256");
+    if (rows == 0) return EDB200_OK;
+    if (x == nullptr || q == nullptr || scale == nullptr) return fail(EDB200_ERR_INVALID, "quantize_fp8: null argument");
+    if ((rows > 1 && (ldx < k || ldq < k)) || (rows > block_rows && ld_scale < (k + 127) / 128)) {
+        return fail(EDB200_ERR_INVALID, "quantize_fp8: ldx and ldq must hold k columns, ld_scale ceil(k / 128)");
+    }
+    const uintptr_t esz = x_dtype == EDB200_TYPE_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(x) % esz || (reinterpret_cast<uintptr_t>(scale) & 3u)) {
+        return fail(EDB200_ERR_INVALID, "quantize_fp8: x and scale must be aligned to their elements");
+    }
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    uint8_t* qb = static_cast<uint8_t*>(q);
+    ProfScope prof(s, PROF_ELEMENTWISE, 0.0, (double)rows * (double)k * (double)(esz + 1));
+    if (x_dtype == EDB200_TYPE_F32) return f8q::launch(static_cast<const float*>(x), ldx, rows, k, block_rows, qb, ldq, scale, ld_scale, s);
+    if (x_dtype == EDB200_TYPE_F16) return f8q::launch(static_cast<const __half*>(x), ldx, rows, k, block_rows, qb, ldq, scale, ld_scale, s);
+    return f8q::launch(static_cast<const __nv_bfloat16*>(x), ldx, rows, k, block_rows, qb, ldq, scale, ld_scale, s);
+}

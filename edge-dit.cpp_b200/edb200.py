@@ -14,8 +14,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libedb200.so")
 
 OK = 0
-TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K, TYPE_I8, TYPE_BF16 = 0, 1, 8, 12, 24, 30
-ACT_NONE, ACT_GELU_TANH, ACT_SILU = 0, 1, 2
+TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K, TYPE_I8, TYPE_BF16, TYPE_F8_E4M3 = 0, 1, 8, 12, 24, 30, 128
+ACT_NONE, ACT_GELU_TANH, ACT_SILU, ACT_GELU_ERF = 0, 1, 2, 3
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_NTK, ROPE_SCALE_YARN = 0, 1, 2, 3
 SPLIT_K_NEVER, SPLIT_K_UNORDERED = 0, 1
 
 c_i64 = C.c_int64
@@ -39,6 +42,38 @@ class QkPack(C.Structure):
         ("pe", c_vp), ("tok_off", c_i64), ("l_total", c_i64), ("q_out", c_vp), ("k_out", c_vp), ("v_out", c_vp),
         ("peers", c_vp),
     ]
+
+
+class Fp8WeightDesc(C.Structure):
+    """edb200_fp8_weight_t"""
+    _fields_ = [("w", c_vp), ("scale", c_vp), ("n", c_i64), ("k", c_i64), ("ldw", c_i64), ("ld_scale", c_i64)]
+
+
+class BlockNormDesc(C.Structure):
+    """edb200_block_norm_t"""
+    _fields_ = [
+        ("rows", c_i64), ("h", c_i64), ("x", c_vp), ("ldx", c_i64), ("residual", c_vp), ("ld_res", c_i64), ("y", c_vp),
+        ("ldy", c_i64), ("z", c_vp), ("ldz", c_i64), ("z_scale", c_vp), ("ld_z_scale", c_i64), ("gate", c_vp),
+        ("scale", c_vp), ("shift", c_vp), ("ld_mod", c_i64), ("rows_per_mod", c_i64), ("post_weight", c_vp),
+        ("post_bias", c_vp), ("pre_weight", c_vp), ("pre_bias", c_vp), ("residual_scale", C.c_float),
+        ("post_eps", C.c_float), ("pre_eps", C.c_float), ("x_dtype", C.c_int), ("stream_dtype", C.c_int),
+        ("z_dtype", C.c_int), ("post_norm", C.c_int), ("pre_norm", C.c_int),
+    ]
+
+
+class RopeConfig(C.Structure):
+    """edb200_rope_config_t"""
+    _fields_ = [
+        ("n_axes", C.c_int), ("axes_dim", C.c_int * 4), ("layout", C.c_int), ("scaling", C.c_int), ("theta", C.c_double),
+        ("factor", C.c_double), ("original_length", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double),
+        ("attention_factor", C.c_double),
+    ]
+
+
+class RopeTensor(C.Structure):
+    """edb200_rope_tensor_t"""
+    _fields_ = [("in_", c_vp), ("out", c_vp), ("in_token", c_i64), ("in_head", c_i64), ("out_token", c_i64),
+                ("out_head", c_i64), ("heads", C.c_int)]
 
 
 class QwenConfig(C.Structure):
@@ -147,6 +182,14 @@ _SIGS = {
     "edb200_cast": (C.c_int, [c_vp, C.c_int, c_vp, C.c_int, c_i64, c_vp]),
     "edb200_attention_f16": (C.c_int, [c_vp, c_vp, c_vp, C.c_int, c_i64, c_i64, C.c_int, C.c_float, c_vp, C.c_int,
                                        c_i64, c_vp]),
+    "edb200_quantize_fp8": (C.c_int, [c_vp, C.c_int, c_i64, c_i64, c_i64, C.c_int, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "edb200_mul_mat_fp8": (C.c_int, [C.POINTER(Fp8WeightDesc), c_vp, c_vp, c_i64, c_i64, c_i64, C.POINTER(Epilogue), c_vp,
+                                     c_i64, c_vp]),
+    "edb200_block_norm": (C.c_int, [C.POINTER(BlockNormDesc), c_vp]),
+    "edb200_rope_create": (C.c_int, [C.POINTER(RopeConfig), C.POINTER(c_vp)]),
+    "edb200_rope_destroy": (None, [c_vp]),
+    "edb200_rope_apply": (C.c_int, [c_vp, C.POINTER(RopeTensor), C.POINTER(RopeTensor), C.c_int, C.c_int, c_i64, c_vp,
+                                    C.c_int, c_vp]),
     "edb200_sage_scratch_bytes": (c_i64, [C.c_int, c_i64, C.c_int]),
     "edb200_sage_scratch_layout": (C.c_int, [C.c_int, c_i64, C.c_int, C.POINTER(c_i64), C.POINTER(C.c_int)]),
     "edb200_sage_quantize_qk": (C.c_int, [c_vp, c_vp, C.c_int, c_i64, C.c_int, C.c_int, c_vp, c_i64, c_vp]),
@@ -324,9 +367,15 @@ def ptr(t):
     return None if t is None else c_vp(t.data_ptr())
 
 
+_DTYPE_IDS = {}
+
+
 def torch_dtype_id(t) -> int:
-    import torch
-    return {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}[t.dtype]
+    if not _DTYPE_IDS:
+        import torch
+        _DTYPE_IDS.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16,
+                           torch.float8_e4m3fn: TYPE_F8_E4M3})
+    return _DTYPE_IDS[t.dtype]
 
 
 def current_stream():
@@ -372,6 +421,167 @@ def make_epilogue(out, bias=None, act=ACT_NONE, residual=None, gate=None, split_
 def mul_mat_q(w: QWeight, x, ep: Epilogue):
     check(lib().edb200_mul_mat_q(w.handle, ptr(x), torch_dtype_id(x), x.shape[0], x.stride(0), C.byref(ep),
                                  current_stream()))
+
+
+def _on_device(*tensors):
+    """Every tensor lies on the current device: the library launches there, on its current stream."""
+    import torch
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"tensor on {t.device}, current device is cuda:{here}")
+
+
+def _rows_of(t, what):
+    """[rows, columns] with neighbouring columns: the row stride in elements."""
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{what} must be two-dimensional with contiguous rows")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _held(t, what, dtype, *shape):
+    """`t` (if any) holds `shape` values of `dtype` and lies contiguously."""
+    if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous()):
+        raise ValueError(f"{what} must be contiguous {dtype} of shape {shape}")
+
+
+def quantize_fp8(x, q, scale, block_rows=1):
+    """q (float8_e4m3fn, like x [rows, k]) and scale (float32 [ceil(rows / block_rows), ceil(k / 128)]) of x:
+    edb200_quantize_fp8 on the current stream."""
+    rows, k = x.shape
+    if tuple(q.shape) != (rows, k) or torch_dtype_id(q) != TYPE_F8_E4M3:
+        raise ValueError("quantize_fp8: q must be float8_e4m3fn of x's shape")
+    if torch_dtype_id(scale) != TYPE_F32 or tuple(scale.shape) != (-(-rows // block_rows), -(-k // 128)):
+        raise ValueError("quantize_fp8: scale must be float32 [ceil(rows / block_rows), ceil(k / 128)]")
+    _on_device(x, q, scale)
+    check(lib().edb200_quantize_fp8(ptr(x), torch_dtype_id(x), _rows_of(x, "x"), rows, k, block_rows, ptr(q),
+                                    _rows_of(q, "q"), ptr(scale), _rows_of(scale, "scale"), current_stream()))
+
+
+class Fp8Weight:
+    """An e4m3 weight [n, k] with scale [ceil(n / 128), ceil(k / 128)] as edb200_fp8_weight_t; keeps both tensors alive."""
+
+    def __init__(self, w, scale):
+        n, k = w.shape
+        if torch_dtype_id(w) != TYPE_F8_E4M3 or torch_dtype_id(scale) != TYPE_F32:
+            raise ValueError("Fp8Weight: w must be float8_e4m3fn and scale float32")
+        if tuple(scale.shape) != (-(-n // 128), -(-k // 128)):
+            raise ValueError("Fp8Weight: scale must be [ceil(n / 128), ceil(k / 128)]")
+        self.w, self.scale = w, scale
+        self.n, self.k = n, k
+        ldw = w.stride(0) if n > 1 else -(-k // 16) * 16
+        self.desc = Fp8WeightDesc(w.data_ptr(), scale.data_ptr(), n, k, ldw, _rows_of(scale, "scale"))
+
+
+def mul_mat_fp8(w: Fp8Weight, x, x_scale, ep: Epilogue, out_scale=None):
+    """edb200_mul_mat_fp8 on the current stream: x float8_e4m3fn [m, k], x_scale float32 [m, ceil(k / 128)], ep from
+    make_epilogue; out_scale float32 [m, ceil(n / 128)] where the epilogue's output is float8_e4m3fn."""
+    m, k = x.shape
+    kb = -(-k // 128)
+    if torch_dtype_id(x) != TYPE_F8_E4M3 or k != w.k:
+        raise ValueError(f"mul_mat_fp8: x must be float8_e4m3fn with {w.k} columns")
+    if torch_dtype_id(x_scale) != TYPE_F32 or tuple(x_scale.shape) != (m, kb):
+        raise ValueError("mul_mat_fp8: x_scale must be float32 [m, ceil(k / 128)]")
+    if out_scale is not None and (torch_dtype_id(out_scale) != TYPE_F32 or tuple(out_scale.shape) != (m, -(-w.n // 128))):
+        raise ValueError("mul_mat_fp8: out_scale must be float32 [m, ceil(n / 128)]")
+    _on_device(x, x_scale, w.w, w.scale, out_scale)
+    ldx = x.stride(0) if m > 1 else -(-k // 16) * 16
+    check(lib().edb200_mul_mat_fp8(C.byref(w.desc), ptr(x), ptr(x_scale), m, ldx, _rows_of(x_scale, "x_scale"),
+                                   C.byref(ep), ptr(out_scale),
+                                   _rows_of(out_scale, "out_scale") if out_scale is not None else 0, current_stream()))
+
+
+def block_norm(residual, y=None, z=None, z_scale=None, x=None, gate=None, residual_scale=1.0, post_norm=NORM_NONE,
+               post_weight=None, post_bias=None, post_eps=1e-6, pre_norm=NORM_NONE, pre_weight=None, pre_bias=None,
+               pre_eps=1e-6, scale=None, shift=None, rows_per_mod=0):
+    """edb200_block_norm on the current stream: y = residual_scale * residual + gate * post(x) and
+    z = pre(y) * (1 + scale) + shift over rows [rows, h].  gate, scale and shift are float32 [groups, h] (or [h]), one
+    row for each rows_per_mod rows (0: one for all); z_scale with a float8_e4m3fn z."""
+    import torch
+    rows, h = residual.shape
+    d = BlockNormDesc()
+    d.rows, d.h = rows, h
+    for t, what in ((x, "x"), (y, "y"), (z, "z")):
+        if t is not None and tuple(t.shape) != (rows, h):
+            raise ValueError(f"block_norm: {what} must have residual's shape")
+    d.residual, d.ld_res, d.stream_dtype = residual.data_ptr(), _rows_of(residual, "residual"), torch_dtype_id(residual)
+    if x is not None:
+        d.x, d.ldx, d.x_dtype = x.data_ptr(), _rows_of(x, "x"), torch_dtype_id(x)
+    if y is not None:
+        if y.dtype != residual.dtype:
+            raise ValueError("block_norm: y must have residual's type")
+        d.y, d.ldy = y.data_ptr(), _rows_of(y, "y")
+    if z is not None:
+        d.z, d.ldz, d.z_dtype = z.data_ptr(), _rows_of(z, "z"), torch_dtype_id(z)
+    if z_scale is not None:
+        if z_scale.dtype != torch.float32 or tuple(z_scale.shape) != (rows, -(-h // 128)):
+            raise ValueError("block_norm: z_scale must be float32 [rows, ceil(h / 128)]")
+        d.z_scale, d.ld_z_scale = z_scale.data_ptr(), _rows_of(z_scale, "z_scale")
+    groups = -(-rows // rows_per_mod) if rows_per_mod else 1
+    ld = None
+    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+        if t is None:
+            continue
+        m = t if t.dim() == 2 else t[None]
+        if m.dtype != torch.float32 or m.dim() != 2 or m.shape[1] != h or m.shape[0] < groups:
+            raise ValueError(f"block_norm: {name} must be float32 [{groups}, {h}]")
+        at = _rows_of(m, name)
+        if groups > 1 and ld is not None and at != ld:
+            raise ValueError("block_norm: gate, scale and shift must share one row stride")
+        ld = at
+        setattr(d, name, t.data_ptr())
+    d.ld_mod, d.rows_per_mod = ld or 0, rows_per_mod
+    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight), ("pre_bias", pre_bias)):
+        if t is not None:
+            _held(t, name, torch.float32, h)
+            setattr(d, name, t.data_ptr())
+    d.residual_scale, d.post_eps, d.pre_eps, d.post_norm, d.pre_norm = residual_scale, post_eps, pre_eps, post_norm, pre_norm
+    _on_device(residual, x, y, z, z_scale, gate, scale, shift, post_weight, post_bias, pre_weight, pre_bias)
+    check(lib().edb200_block_norm(C.byref(d), current_stream()))
+
+
+class Rope:
+    """Owns an edb200_rope_t: the frequencies of rotary positions over one to four axes."""
+
+    def __init__(self, axes_dim, theta=10000.0, layout=ROPE_INTERLEAVED, scaling=ROPE_SCALE_NONE, factor=1.0,
+                 original_length=0.0, beta_fast=0.0, beta_slow=0.0, attention_factor=0.0):
+        self.handle = None
+        if not 1 <= len(axes_dim) <= 4:
+            raise ValueError("Rope: one to four axes")
+        cfg = RopeConfig(len(axes_dim), (C.c_int * 4)(*axes_dim), layout, scaling, theta, factor, original_length,
+                         beta_fast, beta_slow, attention_factor)
+        h = c_vp()
+        check(lib().edb200_rope_create(C.byref(cfg), C.byref(h)))
+        self.handle, self.n_axes, self.width = h, len(axes_dim), sum(axes_dim)
+
+    @staticmethod
+    def _tensor(t, out, like):
+        if t.dim() != 3 or tuple(out.shape) != tuple(t.shape) or out.dtype != t.dtype:
+            raise ValueError("Rope: tensors are [tokens, heads, d_head], out like in")
+        if t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or t.dtype != like.dtype:
+            raise ValueError("Rope: q and k share tokens, d_head and type")
+        if t.shape[2] > 1 and (t.stride(2) != 1 or out.stride(2) != 1):
+            raise ValueError("Rope: channels must be contiguous")
+        return RopeTensor(t.data_ptr(), out.data_ptr(), t.stride(0), t.stride(1), out.stride(0), out.stride(1), t.shape[1])
+
+    def apply(self, positions, q, q_out, k=None, k_out=None, inverse=False):
+        """q_out (and k_out) <- q (and k) [tokens, heads, d_head] turned by positions (int32 [tokens, axes], or None for
+        the token's index) on the current stream; any token and head strides, out may be in itself."""
+        tokens = q.shape[0]
+        if positions is not None:
+            import torch
+            if positions.dtype != torch.int32 or tuple(positions.shape) != (tokens, self.n_axes) or not positions.is_contiguous():
+                raise ValueError(f"Rope: positions must be contiguous int32 [{tokens}, {self.n_axes}]")
+        a = self._tensor(q, q_out, q)
+        b = self._tensor(k, k_out, q) if k is not None else None
+        _on_device(positions, q, q_out, k, k_out)
+        check(lib().edb200_rope_apply(self.handle, C.byref(a), C.byref(b) if b is not None else None, torch_dtype_id(q),
+                                      q.shape[2], tokens, ptr(positions), int(inverse), current_stream()))
+
+    def __del__(self):
+        if getattr(self, "handle", None) and _lib is not None:
+            _lib.edb200_rope_destroy(self.handle)
+            self.handle = None
 
 
 class GGUF:

@@ -44,7 +44,8 @@ enum {
     EDB200_TYPE_Q8_0 = 8,
     EDB200_TYPE_Q4_K = 12,
     EDB200_TYPE_I8 = 24,
-    EDB200_TYPE_BF16 = 30
+    EDB200_TYPE_BF16 = 30,
+    EDB200_TYPE_F8_E4M3 = 128   /* 8-bit float, 4 exponent and 3 mantissa bits, no infinity; ggml has no id for it */
 };
 
 enum { EDB200_SPLIT_K_NEVER = 0, EDB200_SPLIT_K_UNORDERED = 1 };
@@ -346,6 +347,135 @@ EDB200_API edb200_status_t edb200_qk_rownorm_rope_pack(const void* qkv, int in_d
 /* Elementwise dtype conversion (f32/f16/bf16), n a multiple of 4
  * (ggml_cast call sites, e.g. src/dit_models/models/flux.hpp:101-111). */
 EDB200_API edb200_status_t edb200_cast(const void* x, int in_dtype, void* y, int out_dtype, int64_t n, void* stream);
+
+/* ----------------------------------------------- e4m3 linears, scale per block of 128
+ * The block's round in 8-bit floating point: norms around a block that hand on quantised rows, the matrix
+ * product over them, rotary positions for its q and k.  No counterpart in the reference (its linears are
+ * q8_0 / q4_K, edb200_mul_mat_q above); checkpoints that store e4m3 weights with one f32 scale for each
+ * 128 x 128 block run on these directly. */
+
+/* Quantise to e4m3 with one f32 scale for each block of block_rows x 128 values; block_rows is 1 (activations) or
+ * 128 (weights).  For a block whose largest finite magnitude is a (taken as 2^-100 where it is smaller):
+ *   scale = a / 448,   q = e4m3(x * (448 / a)),   both divisions and the product rounded to f32, ties to even.
+ * A value that is not finite becomes NaN and takes no part in a: an infinity is not turned into a number.
+ * x [rows, ldx] f32 / f16 / bf16; q [rows, ldq] bytes; scale [ceil(rows / block_rows), ld_scale], of which
+ * ceil(k / 128) columns are written.  Any rows >= 0, k >= 1, strides and element-aligned addresses; rows that
+ * start on 16-byte boundaries take wide loads.  Columns of q beyond k are left as they were. */
+EDB200_API edb200_status_t edb200_quantize_fp8(const void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t k,
+                                               int block_rows, void* q, int64_t ldq, float* scale, int64_t ld_scale,
+                                               void* stream);
+
+/* An e4m3 weight as it lies in device memory: w [n, ldw] bytes, rows on 16-byte boundaries, and
+ * scale [ceil(n / 128), ld_scale] f32.  Nothing is repacked and nothing is owned. */
+typedef struct {
+    const void* w;
+    const float* scale;
+    int64_t n, k;
+    int64_t ldw;         /* bytes between rows, a multiple of 16 */
+    int64_t ld_scale;    /* floats between rows of scale */
+} edb200_fp8_weight_t;
+
+/* y[m, n] = sum over blocks b of 128 k:  x_scale[m, b] * w.scale[n / 128, b] * (sum over the block of x * w)
+ * (+ bias), then the epilogue's activation and output.  x: [m, ldx] e4m3 bytes, rows on 16-byte boundaries;
+ * x_scale [m, ld_xs] f32.  The products of a block are summed by the tensor cores in f32, the blocks in f32
+ * registers.  Every output is one sum in one order fixed by the sizes: the same bits every run.
+ * The epilogue is that of edb200_mul_mat_q (bias, act with EDB200_ACT_GELU_ERF too, gated residual with f32 out,
+ * f32 / f16 / bf16 out) with these differences: bias and gate need no alignment; out_dtype may be
+ * EDB200_TYPE_F8_E4M3: each row's activated columns are then quantised as edb200_quantize_fp8 does with
+ * block_rows 1, bytes to ep->out and scales to out_scale [m, ld_out_scale], ready to be the next product's x;
+ * split_n, split_k and pack are not available (EDB200_ERR_UNSUPPORTED).  Any m >= 0, n >= 1, k >= 1.
+ * out_scale is NULL for the other output types. */
+EDB200_API edb200_status_t edb200_mul_mat_fp8(const edb200_fp8_weight_t* w, const void* x, const float* x_scale, int64_t m,
+                                              int64_t ldx, int64_t ld_xs, const edb200_epilogue_t* ep, float* out_scale,
+                                              int64_t ld_out_scale, void* stream);
+
+/* Norms before and after a block, its gate and the residual stream in one pass over the rows:
+ *   t = post(x)                                    the block's output, normed where the model norms it
+ *   y = residual_scale * residual + gate * t       the residual stream
+ *   z = pre(y) * (1 + scale) + shift               the next block's input, cast or quantised
+ * post and pre: EDB200_NORM_NONE, EDB200_NORM_LAYER ((v - mean) / sqrt(var + eps)) or EDB200_NORM_RMS
+ * (v / sqrt(mean(v^2) + eps)), times weight plus bias where those are given.  Statistics and sums in f32;
+ * y is rounded to its type once, and z goes on from the unrounded value.
+ *   x NULL: no block output, y = residual_scale * residual.   y NULL: not stored.   z NULL: no second norm.
+ *   gate, scale, shift: f32, one row of h values (ld_mod apart) for each rows_per_mod rows - a batch's samples,
+ *   or single tokens with 1; rows_per_mod 0: one row for all.  NULL: 1, 0, 0.
+ *   z_dtype EDB200_TYPE_F8_E4M3: z is quantised as edb200_quantize_fp8 does with block_rows 1, scales to
+ *   z_scale [rows, ld_z_scale].
+ * y may alias residual or x where type and stride agree.  h up to 16384, any strides; rows of 16-byte aligned
+ * addresses and strides with h a multiple of 8 take wide loads.  Generalises edb200_layernorm_modulate and
+ * edb200_fused_residual_gate, which keep the reference's order of operations bit for bit; this one does not. */
+enum { EDB200_NORM_NONE = 0, EDB200_NORM_LAYER = 1, EDB200_NORM_RMS = 2 };
+typedef struct {
+    int64_t rows, h;
+    const void* x;            /* [rows, ldx] f32 / f16 / bf16, or NULL */
+    int64_t ldx;
+    const void* residual;     /* [rows, ld_res] of stream_dtype */
+    int64_t ld_res;
+    void* y;                  /* [rows, ldy] of stream_dtype, or NULL */
+    int64_t ldy;
+    void* z;                  /* [rows, ldz] of z_dtype, or NULL */
+    int64_t ldz;
+    float* z_scale;           /* [rows, ld_z_scale], with z_dtype EDB200_TYPE_F8_E4M3 */
+    int64_t ld_z_scale;
+    const float* gate;        /* modulation rows, or NULL */
+    const float* scale;
+    const float* shift;
+    int64_t ld_mod;
+    int64_t rows_per_mod;
+    const float* post_weight; /* [h] or NULL */
+    const float* post_bias;
+    const float* pre_weight;
+    const float* pre_bias;
+    float residual_scale, post_eps, pre_eps;
+    int x_dtype, stream_dtype, z_dtype;
+    int post_norm, pre_norm;
+} edb200_block_norm_t;
+EDB200_API edb200_status_t edb200_block_norm(const edb200_block_norm_t* p, void* stream);
+
+/* Rotary positions from position numbers: for models whose channels pair in halves, turn only part of a head, or are
+ * stretched beyond the length they were trained at (edb200_qk_norm_rope_pack takes a dense table instead).
+ * Pair p of the first sum(axes_dim) channels of a head belongs to the axis in whose span it falls and turns by
+ *   positions[token, axis] * theta^(-2 j / axes_dim[axis]),   j = p's place in the span,
+ * computed in 64 bits: angles stay exact to f32 for every 32-bit position, negative ones too.  Channels beyond
+ * the spans pass through.  layout: EDB200_ROPE_INTERLEAVED pairs channels 2p and 2p + 1, EDB200_ROPE_HALF p and
+ * p + half the turned width.  scaling stretches a trained length `original_length` by `factor`:
+ *   LINEAR  divides every frequency by factor;
+ *   NTK     raises theta to theta * factor^(dim / (dim - 2));
+ *   YARN    divides the frequencies that turn less than once in original_length (beta_slow), keeps those that turn more
+ *           than beta_fast times, blends linearly between, and multiplies the turned channels by 0.1 ln(factor) + 1
+ *           (Peng et al., "YaRN", 2023); attention_factor, where it is not 0, replaces that multiplier.
+ * The handle holds the frequencies on the host and may be used from any thread and on any device. */
+enum { EDB200_ROPE_INTERLEAVED = 0, EDB200_ROPE_HALF = 1 };
+enum { EDB200_ROPE_SCALE_NONE = 0, EDB200_ROPE_SCALE_LINEAR = 1, EDB200_ROPE_SCALE_NTK = 2, EDB200_ROPE_SCALE_YARN = 3 };
+typedef struct {
+    int n_axes;              /* 1..4 */
+    int axes_dim[4];         /* channels of each axis, even and positive; at most 256 together */
+    int layout;
+    int scaling;
+    double theta;            /* > 1 */
+    double factor;           /* > 0; 1 or more with YARN (unused without scaling) */
+    double original_length;  /* YARN: > 0 */
+    double beta_fast;        /* YARN: 0 = 32 */
+    double beta_slow;        /* YARN: 0 = 1 */
+    double attention_factor; /* 0 = the scaling's own, else the multiplier of the turned channels */
+} edb200_rope_config_t;
+typedef struct edb200_rope edb200_rope_t;
+EDB200_API edb200_status_t edb200_rope_create(const edb200_rope_config_t* cfg, edb200_rope_t** out);
+EDB200_API void edb200_rope_destroy(edb200_rope_t* r);
+/* One or two tensors (q and k) of f32 / f16 / bf16, [tokens, heads, d_head] in any order: element strides between
+ * tokens and between heads, channels contiguous.  Strides of out laid head-major give attention operands.  out may
+ * be in itself (same strides); otherwise the two do not overlap.  positions: [tokens, n_axes] int32 on the device,
+ * or NULL = the token's index on every axis.  inverse turns back (the gradient of the forward call, multiplier
+ * included).  k with k->in NULL or k NULL: q alone. */
+typedef struct {
+    const void* in;
+    void* out;
+    int64_t in_token, in_head, out_token, out_head;   /* element strides */
+    int heads;
+} edb200_rope_tensor_t;
+EDB200_API edb200_status_t edb200_rope_apply(const edb200_rope_t* r, const edb200_rope_tensor_t* q,
+                                             const edb200_rope_tensor_t* k, int dtype, int d_head, int64_t tokens,
+                                             const int32_t* positions, int inverse, void* stream);
 
 /* -------------------------------------------------------------- attention
  * Non-causal softmax(Q K^T * scale) V.  q [hn, lq, d_head], k/v [hn, lk, d_head]
