@@ -35,7 +35,7 @@ struct Params {
     long long ldo, ld_res, ld_os;
     int M, N, kblocks;
     int act, out_dtype;
-    int m_tiles;
+    int m_tiles, n_tiles, chunk;   // chunk: feature tiles walked together (pair kernel)
     int* err;
 };
 
@@ -50,19 +50,37 @@ __device__ __forceinline__ void mma_f8_ss(uint32_t tmem_d, uint64_t adesc, uint6
         : "memory");
 }
 
-// acc[i] += s * r[i], two elements an instruction.
-template <int N>
-__device__ __forceinline__ void promote(float (&acc)[N], int at, const uint32_t (&r)[32], float s) {
+// The same over a CTA pair: 256 tokens (128 in either CTA's tensor memory), B rows 0 .. N/2 - 1 from the leader's
+// shared memory and the rest from the peer's.
+__device__ __forceinline__ void mma_f8_ss_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// acc[i] += s * r[i], two elements an instruction.  The packed form has the scalar one's rate (2.2 clocks for two) in half
+// the issue slots, and the slots matter more: eight warps of back-to-back scalar FMAs left the issuing warp none, and the
+// tensor pipe stood still until they were done.  Sums are held as register pairs throughout.
+template <int N, int R>
+__device__ __forceinline__ void promote(uint64_t (&acc)[N], int at, const uint32_t (&r)[R], float s) {
     uint64_t ss;
     asm("mov.b64 %0, {%1, %1};" : "=l"(ss) : "f"(s));
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-        uint64_t a, b;
-        asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(acc[at + i]), "f"(acc[at + i + 1]));
-        asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "r"(r[i]), "r"(r[i + 1]));
-        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(b), "l"(ss));
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[at + i]), "=f"(acc[at + i + 1]) : "l"(a));
+    for (int i = 0; i < R / 2; ++i) {
+        uint64_t b;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "r"(r[2 * i]), "r"(r[2 * i + 1]));
+        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[at / 2 + i]) : "l"(b), "l"(ss));
     }
+}
+template <int N>
+__device__ __forceinline__ void unpack_sums(const uint64_t (&sum)[N], float (&v)[2 * N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm("mov.b64 {%0, %1}, %2;" : "=f"(v[2 * i]), "=f"(v[2 * i + 1]) : "l"(sum[i]));
 }
 
 // The activations by exp and one division: gelu_tanh(v) = v / (1 + exp(-2 u)), exact to a few f32 roundings.
@@ -327,9 +345,9 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         const float* xs = P.xs + m * P.ld_xs;
         const float* ws = P.ws + n_tile * P.ld_ws;
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + side * CPT;
-        float acc[CPT];
+        uint64_t sum[CPT / 2];
 #pragma unroll
-        for (int i = 0; i < CPT; ++i) acc[i] = 0.0f;
+        for (int i = 0; i < CPT / 2; ++i) sum[i] = 0;
         float scale = __ldg(xs) * __ldg(ws);
         bool ok = true;
         for (int b = 0; b < P.kblocks; ++b) {
@@ -346,12 +364,14 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buf]);
-            promote(acc, 0, r0, scale);
-            promote(acc, 32, r1, scale);
+            promote(sum, 0, r0, scale);
+            promote(sum, 32, r1, scale);
             scale = next;
         }
         const int nc = n0 + side * CPT;
         float amax = 0.0f;
+        float acc[CPT];
+        unpack_sums(sum, acc);
         if (ok) bias_act(acc, s_bias + side * CPT, P.act);
         if (P.out_dtype == EDB200_TYPE_F8_E4M3) {   // uniform: the row's other half lies in the other warp group
             s_max[side * 128 + row] = row_magnitude(acc, nc, P.N);
@@ -369,6 +389,288 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     if (warp == 1) {
         tc_fence_after_sync();
         tmem_dealloc(tmem_base, 256);
+    }
+}
+
+// ------------------------------------------------------ CTA pairs: 256 tokens x 256 features, one pair per two SMs
+// The leader's MMAs span both CTAs (cta_group::2): each stages its own 128 tokens and half of the 256 features, so an
+// SM takes in 32 KB for 512 clocks of tensor work.  The two 128-feature halves of a block are MMAs and accumulators of
+// their own: all 512 tensor-memory columns hold [half][2 alternating][128], and a half's accumulator is due again only
+// three MMA groups (768 clocks) after it was finished - with one 256-column pair of accumulators the tensor pipe waited
+// for the reading of the last one half of the time.  Each of eight promotion warps owns 32 tokens x one half, which is
+// one weight block and, for e4m3 output, one quantisation block.
+// Each half has an issuer of its own (warps 1 and 2 of the leader): waiting, issuing and committing are a chain of about
+// 250 clocks a group for one thread, twice that per block for a common one.
+// Warp 3 brings the scales, eight blocks of the CTA's 128 rows at a time, two groups in shared memory.  The promotion
+// warps touch no global memory while they add: with one load in flight each of their tensor-memory reads waited for
+// it (1060 clocks a block instead of 650).
+// Signals across the pair: the peer's warp 1 passes its full barriers on to the leader's (two arrivals there: own copies,
+// peer's); acc_empty counts the promotion warps of both CTAs; the commits arrive in both.
+namespace pair {
+constexpr int STAGES = 5;
+constexpr int A_BYTES = 128 * BK, B_HALF = 64 * BK, STAGE_BYTES = A_BYTES + 2 * B_HALF;
+constexpr int WARPS = 8;
+constexpr int CPT = 128;
+constexpr int OFF_STAGE = STAGES * STAGE_BYTES;
+constexpr int OFF_VEC = OFF_STAGE + WARPS * 32 * PITCH * 4;     // [2 tiles][2 halves][bias 128, gate 128]
+constexpr int SCALE_WORDS = 128 * 9 + 16;                        // a group: [row][8 blocks + 1], then ws [half][8]
+constexpr int OFF_SCALE = OFF_VEC + 2 * 2 * 256 * 4;
+constexpr int OFF_BAR = OFF_SCALE + 2 * SCALE_WORDS * 4;
+constexpr int SMEM_BYTES = OFF_BAR + 256 + 1024;
+constexpr int THREADS = 32 * (WARPS + 4);                       // registers move in groups of four warps
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory plan");
+}  // namespace pair
+
+__device__ __forceinline__ void pair_tile_at(const Params& P, int t, int& m_tile, int& n_tile) {
+    const int per = P.m_tiles * P.chunk;
+    const int c = t / per, r = t - c * per;
+    const int first = c * P.chunk, width = P.n_tiles - first < P.chunk ? P.n_tiles - first : P.chunk;
+    m_tile = r / width;
+    n_tile = first + r - m_tile * width;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
+fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                const __grid_constant__ Params P) {
+    using namespace pair;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + OFF_BAR);   // [STAGES]
+    uint64_t* empty = full + STAGES;                                // [STAGES]
+    uint64_t* acc_full = empty + STAGES;                            // [half][2]
+    uint64_t* acc_empty = acc_full + 4;                             // [half][2]  (the leader's are used)
+    uint64_t* sc_full = acc_empty + 4;                              // [2]
+    uint64_t* sc_empty = sc_full + 2;                               // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(cluster_ctarank());
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int tiles = P.m_tiles * P.n_tiles;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(&full[i], rank == 0 ? 2 : 1);
+            mbar_init(&empty[i], 2);                  // either half's MMAs have read the stage
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], WARPS);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sc_full[i], 1);
+            mbar_init(&sc_empty[i], WARPS);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&map_x);
+        tma_prefetch_desc(&map_w);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();     // the peer's barriers are initialised before anything arrives on them
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+
+    // 168 registers a thread at launch (384 threads); the promotion warps take what the others give up:
+    // 256 x 224 + 128 x 56 = 384 x 168
+    if (warp >= 4) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int quarter = warp & 3, side = (warp - 4) >> 2;
+        const int row = quarter * 32 + lane;
+        float* stage = reinterpret_cast<float*>(smem + OFF_STAGE) + (warp - 4) * 32 * PITCH;
+        const float* scales = reinterpret_cast<const float*>(smem + OFF_SCALE);
+        uint32_t sg = 0;   // group of scales, over all tiles
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + side * 256;
+        const uint32_t free0 = leader_address(&acc_empty[2 * side]), free1 = leader_address(&acc_empty[2 * side + 1]);
+        uint32_t g = 0, parity = 0;
+        bool ok = true;
+        for (int t = first; ok && t < tiles; t += step, parity ^= 1u) {
+            int m_tile, n_tile;
+            pair_tile_at(P, t, m_tile, n_tile);
+            const int m_first = m_tile * 256 + rank * 128 + quarter * 32;   // the warp's rows
+            const int nc = n_tile * 256 + side * CPT;                       // the thread's columns
+            const bool n_ok = nc + row < P.N;
+            const float bias_v = (P.bias != nullptr && n_ok) ? __ldg(P.bias + nc + row) : 0.0f;
+            const float gate_v = (P.gate != nullptr && n_ok) ? __ldg(P.gate + nc + row) : 0.0f;
+            uint64_t sum[CPT / 2];
+#pragma unroll
+            for (int i = 0; i < CPT / 2; ++i) sum[i] = 0;
+            // One block's reading runs into the next one's: the barrier of block b + 1 is looked at and its first columns
+            // are under way before block b's last products are added.
+            ok = __all_sync(0xffffffffu, mbar_wait(&sc_full[sg & 1u], (sg >> 1) & 1u, abort_flag, P.err));
+            if (!ok) break;
+            const float* sc = scales + (sg & 1u) * SCALE_WORDS;
+            float scale = sc[row * 9] * sc[128 * 9 + side * 8];
+            uint32_t r0[32], r1[32];
+            ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[2 * side + (g & 1u)], (g >> 1) & 1u, abort_flag, P.err));
+            if (!ok) break;
+            tc_fence_after_sync();
+            tmem_ld_32x32b_x32(taddr + (g & 1u) * 128, r0);
+            for (int b = 0; b < P.kblocks; ++b, ++g) {
+                const uint32_t at = taddr + (g & 1u) * 128;
+                const uint32_t nbuf = (g + 1) & 1u, nph = ((g + 1) >> 1) & 1u;
+                const float s = scale;
+                tmem_wait_ld();
+                tmem_ld_32x32b_x32(at + 32, r1);
+                promote(sum, 0, r0, s);
+                tmem_wait_ld();
+                tmem_ld_32x32b_x32(at + 64, r0);
+                promote(sum, 32, r1, s);
+                tmem_wait_ld();
+                tmem_ld_32x32b_x32(at + 96, r1);
+                const bool there = mbar_test(&acc_full[2 * side + nbuf], nph);
+                promote(sum, 64, r0, s);
+                if (((b + 1) & 7) == 0 || b + 1 == P.kblocks) {   // the group is read
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sc_empty[sg & 1u]);
+                    ++sg;
+                    sc = scales + (sg & 1u) * SCALE_WORDS;
+                    if (b + 1 < P.kblocks) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&sc_full[sg & 1u], (sg >> 1) & 1u, abort_flag, P.err));
+                        if (!ok) break;
+                    }
+                }
+                scale = sc[row * 9 + ((b + 1) & 7)] * sc[128 * 9 + side * 8 + ((b + 1) & 7)];   // unused after the last block
+                tmem_wait_ld();
+                tc_fence_before_sync();
+                if (lane == 0) mbar_arrive_relaxed((g & 1u) ? free1 : free0);
+                if (b + 1 < P.kblocks) {
+                    if (!__all_sync(0xffffffffu, there)) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[2 * side + nbuf], nph, abort_flag, P.err));
+                        if (!ok) break;
+                    }
+                    tc_fence_after_sync();
+                    tmem_ld_32x32b_x32(taddr + nbuf * 128, r0);
+                }
+                promote(sum, 96, r1, s);
+            }
+            if (!ok) break;
+            float* vec = reinterpret_cast<float*>(smem + OFF_VEC) + (parity * 2 + side) * 256;
+            vec[row] = bias_v;
+            vec[128 + row] = gate_v;
+            named_bar_sync(1 + side, 128);
+            float acc[CPT];
+            unpack_sums(sum, acc);
+            bias_act(acc, vec, P.act);
+            float amax = 0.0f;
+            if (P.out_dtype == EDB200_TYPE_F8_E4M3) amax = row_magnitude(acc, nc, P.N);
+            store_rows(P, acc, m_first, nc, lane, stage, vec + 128, amax);
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0) {
+            uint32_t s = 0, ph = 0;
+            bool ok = true;
+            for (int t = first; ok && t < tiles; t += step) {
+                int m_tile, n_tile;
+                pair_tile_at(P, t, m_tile, n_tile);
+                const int m0 = m_tile * 256 + rank * 128, n0 = n_tile * 256 + rank * 64;
+                for (int b = 0; b < P.kblocks; ++b) {
+                    if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, P.err)) {
+                        ok = false;
+                        break;
+                    }
+                    if (elect_one()) {
+                        uint8_t* stage = smem + s * STAGE_BYTES;
+                        mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
+                        tma_load_2d(stage, &map_x, &full[s], b * BK, m0);
+                        tma_load_2d(stage + A_BYTES, &map_w, &full[s], b * BK, n0);
+                        tma_load_2d(stage + A_BYTES + B_HALF, &map_w, &full[s], b * BK, n0 + 128);
+                    }
+                    __syncwarp();
+                    if (++s == STAGES) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+        } else if (warp <= 2 && rank == 0) {
+            const int half = warp - 1;
+            const uint32_t idesc = make_idesc(kDFmtF32, kFmtE4M3, kFmtE4M3, 0, 0, 256, 128);
+            const uint64_t a_desc0 = make_smem_desc_sw128(smem_u32(smem), 16, 1024);
+            const uint64_t b_desc0 = make_smem_desc_sw128(smem_u32(smem) + A_BYTES + half * B_HALF, 16, 1024);
+            const int blocks = first < tiles ? ((tiles - first + step - 1) / step) * P.kblocks : 0;
+            uint32_t s = 0, ph = 0;
+            for (int g = 0; g < blocks; ++g) {   // k blocks of all this pair's tiles
+                const uint32_t buf = g & 1u, aph = (g >> 1) & 1u;
+                if (!mbar_wait(&acc_empty[2 * half + buf], aph ^ 1u, abort_flag, P.err)) break;
+                if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
+                tc_fence_after_sync();
+                if (elect_one()) {
+                    const uint32_t d = tmem_base + half * 256 + buf * 128;
+                    const uint32_t off = s * (STAGE_BYTES >> 4);   // descriptors count 16-byte units
+#pragma unroll
+                    for (int j = 0; j < BK / 32; ++j) {
+                        mma_f8_ss_pair(d, a_desc0 + off + 2 * j, b_desc0 + off + 2 * j, idesc, j > 0 ? 1u : 0u);
+                    }
+                    mma_commit_pair(&acc_full[2 * half + buf]);
+                    mma_commit_pair(&empty[s]);
+                }
+                __syncwarp();
+                if (++s == STAGES) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
+        } else if (warp == 3) {
+            const int nb_last = (P.N - 1) >> 7;
+            float* dst0 = reinterpret_cast<float*>(smem + OFF_SCALE);
+            uint32_t sg = 0;
+            bool ok = true;
+            for (int t = first; ok && t < tiles; t += step) {
+                int m_tile, n_tile;
+                pair_tile_at(P, t, m_tile, n_tile);
+                const int m0 = m_tile * 256 + rank * 128;
+                for (int b = 0; b < P.kblocks; b += 8, ++sg) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sc_empty[sg & 1u], ((sg >> 1) & 1u) ^ 1u, abort_flag, P.err));
+                    if (!ok) break;
+                    float* dst = dst0 + (sg & 1u) * SCALE_WORDS;
+                    const int at = b + (lane & 7) < P.kblocks ? b + (lane & 7) : P.kblocks - 1;
+                    if (lane < 16) {
+                        const int nb = 2 * n_tile + (lane >> 3);
+                        dst[128 * 9 + lane] = __ldg(P.ws + static_cast<long long>(nb < nb_last ? nb : nb_last) * P.ld_ws + at);
+                    }
+#pragma unroll 8
+                    for (int i = 0; i < 32; ++i) {   // four rows of eight blocks a load; rows past the end follow the last one
+                        const int r = 4 * i + (lane >> 3);
+                        const int m = m0 + r < P.M ? m0 + r : P.M - 1;
+                        dst[r * 9 + (lane & 7)] = __ldg(P.xs + m * P.ld_xs + at);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sc_full[sg & 1u]);
+                }
+            }
+        } else if (warp == 1) {
+            const int blocks = first < tiles ? ((tiles - first + step - 1) / step) * P.kblocks : 0;
+            uint32_t s = 0, ph = 0;
+            for (int g = 0; g < blocks; ++g) {
+                if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
+                if (elect_one()) mbar_arrive_leader(&full[s]);
+                __syncwarp();
+                if (++s == STAGES) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (*abort_flag) {
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);   // let copies and MMAs in flight land
+        __syncthreads();
+    }
+    cluster_sync_all();     // neither CTA leaves while the other may signal it or the pair's MMAs read its memory
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem_base, 512);
     }
 }
 
@@ -400,6 +702,39 @@ static edb200_status_t launch_tile(const edb200_fp8_weight_t& w, const void* x, 
     const int64_t tiles = (int64_t)P.m_tiles * ((w.n + 127) / 128);
     if (tiles > 0x7fffffff) return fail(EDB200_ERR_UNSUPPORTED, "mul_mat_fp8: too many output tiles");
     fp8_tile_kernel<<<static_cast<unsigned>(tiles), tile::THREADS, tile::SMEM_BYTES, s>>>(map_x, map_w, P);
+    count_launch();
+    return check_cuda(cudaGetLastError(), "mul_mat_fp8 launch");
+}
+
+static edb200_status_t launch_pair(const edb200_fp8_weight_t& w, const void* x, int64_t m, int64_t ldx, Params& P, cudaStream_t s) {
+    CUtensorMap map_x, map_w;
+    EDB_TRY(operand_map(&map_x, x, w.k, m, ldx, 128));
+    EDB_TRY(operand_map(&map_w, w.w, w.k, w.n, w.ldw, 64));
+    static bool done[64] = {false};
+    EDB_TRY(allow_smem(fp8_pair_kernel, pair::SMEM_BYTES, done));
+    static int max_pairs = 0;   // CTA pairs that can be resident at once
+    if (max_pairs == 0) {
+        cudaLaunchConfig_t cfg;
+        memset(&cfg, 0, sizeof(cfg));
+        cfg.gridDim = dim3(static_cast<unsigned>(sm_count() & ~1), 1, 1);
+        cfg.blockDim = dim3(pair::THREADS, 1, 1);
+        cfg.dynamicSmemBytes = pair::SMEM_BYTES;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, fp8_pair_kernel, &cfg) != cudaSuccess || n <= 0) {
+            (void)cudaGetLastError();
+            n = sm_count() / 2;
+        }
+        max_pairs = n < sm_count() / 2 ? n : sm_count() / 2;
+    }
+    P.m_tiles = static_cast<int>((m + 255) / 256);
+    P.n_tiles = static_cast<int>((w.n + 255) / 256);
+    // feature tiles walked together: their weights, read again for every token tile, stay within about a third of L2
+    const int64_t ch = (44ll << 20) / (256 * w.k);
+    P.chunk = static_cast<int>(ch < 1 ? 1 : ch < P.n_tiles ? ch : P.n_tiles);
+    const int64_t tiles = (int64_t)P.m_tiles * P.n_tiles;
+    if (tiles > 0x3fffffff) return fail(EDB200_ERR_UNSUPPORTED, "mul_mat_fp8: too many output tiles");
+    const unsigned grid = 2u * static_cast<unsigned>(tiles < max_pairs ? tiles : max_pairs);
+    fp8_pair_kernel<<<grid, pair::THREADS, pair::SMEM_BYTES, s>>>(map_x, map_w, P);
     count_launch();
     return check_cuda(cudaGetLastError(), "mul_mat_fp8 launch");
 }
@@ -475,5 +810,6 @@ extern "C" edb200_status_t edb200_mul_mat_fp8(const edb200_fp8_weight_t* w, cons
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof(s, PROF_GEMM, 2.0 * (double)m * (double)w->n * (double)w->k,
                    (double)w->n * (double)w->k + (double)m * (double)w->k + (double)m * (double)w->n * esz);
+    if (((m + 255) / 256) * ((w->n + 255) / 256) >= 37) return f8g::launch_pair(*w, x, m, ldx, P, s);
     return f8g::launch_tile(*w, x, m, ldx, P, s);
 }

@@ -72,6 +72,21 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // Bounded wait.  `abort_flag` lives in shared memory; once any thread of the
 // CTA has set it every later wait returns at once.  `err` is a global status
 // word read by the host after the launch.
@@ -332,6 +347,17 @@ __device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(smem_u32(bar)));
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+}
+
+// The leader's address of a barrier, and an arrival there without release ordering: for a signal behind which only tensor
+// memory lies that this thread has read (tcgen05.wait::ld and tcgen05.fence::before_thread_sync come first).
+__device__ __forceinline__ uint32_t leader_address(uint64_t* bar) {
+    uint32_t remote;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(smem_u32(bar)));
+    return remote;
+}
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t cluster_address) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_address) : "memory");
 }
 
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t ncols) {

@@ -423,39 +423,42 @@ def mul_mat_q(w: QWeight, x, ep: Epilogue):
                                  current_stream()))
 
 
-def _on_device(*tensors):
-    """Every tensor lies on the current device: the library launches there, on its current stream."""
+def _launch_stream(*tensors):
+    """The current stream, as the C entries take it.  Every tensor must lie on the current device: the library
+    launches there."""
     import torch
     here = torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != here:
             raise ValueError(f"tensor on {t.device}, current device is cuda:{here}")
+    return torch.cuda.current_stream(here).cuda_stream
 
 
 def _rows_of(t, what):
-    """[rows, columns] with neighbouring columns: the row stride in elements."""
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+    """[rows, columns] with neighbouring columns: the row stride in elements (a single row's is not used)."""
+    s = t.stride()
+    if len(s) != 2 or (s[1] != 1 and t.shape[1] > 1):
         raise ValueError(f"{what} must be two-dimensional with contiguous rows")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return s[0]
 
 
-def _held(t, what, dtype, *shape):
-    """`t` (if any) holds `shape` values of `dtype` and lies contiguously."""
-    if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous()):
-        raise ValueError(f"{what} must be contiguous {dtype} of shape {shape}")
+def _scale_rows(t, rows, blocks, what):
+    if t.shape != (rows, blocks) or torch_dtype_id(t) != TYPE_F32:
+        raise ValueError(f"{what} must be float32 [{rows}, {blocks}]")
+    return _rows_of(t, what)
 
 
 def quantize_fp8(x, q, scale, block_rows=1):
     """q (float8_e4m3fn, like x [rows, k]) and scale (float32 [ceil(rows / block_rows), ceil(k / 128)]) of x:
     edb200_quantize_fp8 on the current stream."""
     rows, k = x.shape
-    if tuple(q.shape) != (rows, k) or torch_dtype_id(q) != TYPE_F8_E4M3:
+    if q.shape != x.shape or torch_dtype_id(q) != TYPE_F8_E4M3:
         raise ValueError("quantize_fp8: q must be float8_e4m3fn of x's shape")
-    if torch_dtype_id(scale) != TYPE_F32 or tuple(scale.shape) != (-(-rows // block_rows), -(-k // 128)):
-        raise ValueError("quantize_fp8: scale must be float32 [ceil(rows / block_rows), ceil(k / 128)]")
-    _on_device(x, q, scale)
-    check(lib().edb200_quantize_fp8(ptr(x), torch_dtype_id(x), _rows_of(x, "x"), rows, k, block_rows, ptr(q),
-                                    _rows_of(q, "q"), ptr(scale), _rows_of(scale, "scale"), current_stream()))
+    lds = _scale_rows(scale, -(-rows // block_rows), -(-k // 128), "quantize_fp8: scale")
+    st = lib().edb200_quantize_fp8(x.data_ptr(), torch_dtype_id(x), _rows_of(x, "x"), rows, k, block_rows, q.data_ptr(),
+                                   _rows_of(q, "q"), scale.data_ptr(), lds, _launch_stream(x, q, scale))
+    if st:
+        check(st)
 
 
 class Fp8Weight:
@@ -463,32 +466,27 @@ class Fp8Weight:
 
     def __init__(self, w, scale):
         n, k = w.shape
-        if torch_dtype_id(w) != TYPE_F8_E4M3 or torch_dtype_id(scale) != TYPE_F32:
-            raise ValueError("Fp8Weight: w must be float8_e4m3fn and scale float32")
-        if tuple(scale.shape) != (-(-n // 128), -(-k // 128)):
-            raise ValueError("Fp8Weight: scale must be [ceil(n / 128), ceil(k / 128)]")
-        self.w, self.scale = w, scale
-        self.n, self.k = n, k
-        ldw = w.stride(0) if n > 1 else -(-k // 16) * 16
-        self.desc = Fp8WeightDesc(w.data_ptr(), scale.data_ptr(), n, k, ldw, _rows_of(scale, "scale"))
+        if torch_dtype_id(w) != TYPE_F8_E4M3:
+            raise ValueError("Fp8Weight: w must be float8_e4m3fn")
+        lds = _scale_rows(scale, -(-n // 128), -(-k // 128), "Fp8Weight: scale")
+        self.w, self.scale, self.n, self.k = w, scale, n, k
+        self.desc = Fp8WeightDesc(w.data_ptr(), scale.data_ptr(), n, k, _rows_of(w, "Fp8Weight: w"), lds)
+        self.ref = C.byref(self.desc)
 
 
 def mul_mat_fp8(w: Fp8Weight, x, x_scale, ep: Epilogue, out_scale=None):
     """edb200_mul_mat_fp8 on the current stream: x float8_e4m3fn [m, k], x_scale float32 [m, ceil(k / 128)], ep from
     make_epilogue; out_scale float32 [m, ceil(n / 128)] where the epilogue's output is float8_e4m3fn."""
     m, k = x.shape
-    kb = -(-k // 128)
-    if torch_dtype_id(x) != TYPE_F8_E4M3 or k != w.k:
+    if k != w.k or torch_dtype_id(x) != TYPE_F8_E4M3:
         raise ValueError(f"mul_mat_fp8: x must be float8_e4m3fn with {w.k} columns")
-    if torch_dtype_id(x_scale) != TYPE_F32 or tuple(x_scale.shape) != (m, kb):
-        raise ValueError("mul_mat_fp8: x_scale must be float32 [m, ceil(k / 128)]")
-    if out_scale is not None and (torch_dtype_id(out_scale) != TYPE_F32 or tuple(out_scale.shape) != (m, -(-w.n // 128))):
-        raise ValueError("mul_mat_fp8: out_scale must be float32 [m, ceil(n / 128)]")
-    _on_device(x, x_scale, w.w, w.scale, out_scale)
-    ldx = x.stride(0) if m > 1 else -(-k // 16) * 16
-    check(lib().edb200_mul_mat_fp8(C.byref(w.desc), ptr(x), ptr(x_scale), m, ldx, _rows_of(x_scale, "x_scale"),
-                                   C.byref(ep), ptr(out_scale),
-                                   _rows_of(out_scale, "out_scale") if out_scale is not None else 0, current_stream()))
+    ldxs = _scale_rows(x_scale, m, -(-k // 128), "mul_mat_fp8: x_scale")
+    ldos = _scale_rows(out_scale, m, -(-w.n // 128), "mul_mat_fp8: out_scale") if out_scale is not None else 0
+    st = lib().edb200_mul_mat_fp8(w.ref, x.data_ptr(), x_scale.data_ptr(), m, _rows_of(x, "x"), ldxs, C.byref(ep),
+                                  out_scale.data_ptr() if out_scale is not None else None, ldos,
+                                  _launch_stream(x, x_scale, w.w, w.scale, out_scale))
+    if st:
+        check(st)
 
 
 def block_norm(residual, y=None, z=None, z_scale=None, x=None, gate=None, residual_scale=1.0, post_norm=NORM_NONE,
@@ -497,47 +495,49 @@ def block_norm(residual, y=None, z=None, z_scale=None, x=None, gate=None, residu
     """edb200_block_norm on the current stream: y = residual_scale * residual + gate * post(x) and
     z = pre(y) * (1 + scale) + shift over rows [rows, h].  gate, scale and shift are float32 [groups, h] (or [h]), one
     row for each rows_per_mod rows (0: one for all); z_scale with a float8_e4m3fn z."""
-    import torch
-    rows, h = residual.shape
-    d = BlockNormDesc()
-    d.rows, d.h = rows, h
-    for t, what in ((x, "x"), (y, "y"), (z, "z")):
-        if t is not None and tuple(t.shape) != (rows, h):
-            raise ValueError(f"block_norm: {what} must have residual's shape")
-    d.residual, d.ld_res, d.stream_dtype = residual.data_ptr(), _rows_of(residual, "residual"), torch_dtype_id(residual)
+    shape = residual.shape
+    rows, h = shape
+    px = py = pz = pzs = None
+    ldx = ldy = ldz = ldzs = x_id = z_id = 0
+    stream_id = torch_dtype_id(residual)
     if x is not None:
-        d.x, d.ldx, d.x_dtype = x.data_ptr(), _rows_of(x, "x"), torch_dtype_id(x)
+        px, ldx, x_id = x.data_ptr(), _rows_of(x, "x"), torch_dtype_id(x)
     if y is not None:
+        py, ldy = y.data_ptr(), _rows_of(y, "y")
         if y.dtype != residual.dtype:
             raise ValueError("block_norm: y must have residual's type")
-        d.y, d.ldy = y.data_ptr(), _rows_of(y, "y")
     if z is not None:
-        d.z, d.ldz, d.z_dtype = z.data_ptr(), _rows_of(z, "z"), torch_dtype_id(z)
+        pz, ldz, z_id = z.data_ptr(), _rows_of(z, "z"), torch_dtype_id(z)
+    if (x is not None and x.shape != shape) or (y is not None and y.shape != shape) or (z is not None and z.shape != shape):
+        raise ValueError("block_norm: x, y and z must have residual's shape")
     if z_scale is not None:
-        if z_scale.dtype != torch.float32 or tuple(z_scale.shape) != (rows, -(-h // 128)):
-            raise ValueError("block_norm: z_scale must be float32 [rows, ceil(h / 128)]")
-        d.z_scale, d.ld_z_scale = z_scale.data_ptr(), _rows_of(z_scale, "z_scale")
+        pzs, ldzs = z_scale.data_ptr(), _scale_rows(z_scale, rows, -(-h // 128), "block_norm: z_scale")
     groups = -(-rows // rows_per_mod) if rows_per_mod else 1
-    ld = None
-    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+    ld, mod = 0, [None, None, None]
+    for i, t in enumerate((gate, scale, shift)):
         if t is None:
             continue
-        m = t if t.dim() == 2 else t[None]
-        if m.dtype != torch.float32 or m.dim() != 2 or m.shape[1] != h or m.shape[0] < groups:
-            raise ValueError(f"block_norm: {name} must be float32 [{groups}, {h}]")
-        at = _rows_of(m, name)
-        if groups > 1 and ld is not None and at != ld:
+        if t.dim() == 1:
+            t = t[None]
+        if t.shape[1] != h or t.shape[0] < groups or torch_dtype_id(t) != TYPE_F32:
+            raise ValueError(f"block_norm: gate, scale and shift must be float32 [{groups}, {h}]")
+        at = _rows_of(t, "modulation")
+        if groups > 1 and ld and at != ld:
             raise ValueError("block_norm: gate, scale and shift must share one row stride")
-        ld = at
-        setattr(d, name, t.data_ptr())
-    d.ld_mod, d.rows_per_mod = ld or 0, rows_per_mod
-    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight), ("pre_bias", pre_bias)):
+        ld, mod[i] = at, t.data_ptr()
+    affine = [None, None, None, None]
+    for i, t in enumerate((post_weight, post_bias, pre_weight, pre_bias)):
         if t is not None:
-            _held(t, name, torch.float32, h)
-            setattr(d, name, t.data_ptr())
-    d.residual_scale, d.post_eps, d.pre_eps, d.post_norm, d.pre_norm = residual_scale, post_eps, pre_eps, post_norm, pre_norm
-    _on_device(residual, x, y, z, z_scale, gate, scale, shift, post_weight, post_bias, pre_weight, pre_bias)
-    check(lib().edb200_block_norm(C.byref(d), current_stream()))
+            if t.shape != (h,) or torch_dtype_id(t) != TYPE_F32 or not t.is_contiguous():
+                raise ValueError(f"block_norm: weights and biases must be contiguous float32 [{h}]")
+            affine[i] = t.data_ptr()
+    d = BlockNormDesc(rows, h, px, ldx, residual.data_ptr(), _rows_of(residual, "residual"), py, ldy, pz, ldz, pzs, ldzs,
+                      *mod, ld, rows_per_mod, *affine, residual_scale, post_eps, pre_eps, x_id, stream_id, z_id, post_norm,
+                      pre_norm)
+    st = lib().edb200_block_norm(C.byref(d), _launch_stream(residual, x, y, z, z_scale, gate, scale, shift, post_weight,
+                                                            post_bias, pre_weight, pre_bias))
+    if st:
+        check(st)
 
 
 class Rope:
@@ -555,28 +555,34 @@ class Rope:
         self.handle, self.n_axes, self.width = h, len(axes_dim), sum(axes_dim)
 
     @staticmethod
-    def _tensor(t, out, like):
-        if t.dim() != 3 or tuple(out.shape) != tuple(t.shape) or out.dtype != t.dtype:
+    def _tensor(t, out):
+        si, so = t.stride(), out.stride()
+        if len(si) != 3 or out.shape != t.shape or out.dtype != t.dtype:
             raise ValueError("Rope: tensors are [tokens, heads, d_head], out like in")
-        if t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or t.dtype != like.dtype:
-            raise ValueError("Rope: q and k share tokens, d_head and type")
-        if t.shape[2] > 1 and (t.stride(2) != 1 or out.stride(2) != 1):
+        if si[2] != 1 or so[2] != 1:
             raise ValueError("Rope: channels must be contiguous")
-        return RopeTensor(t.data_ptr(), out.data_ptr(), t.stride(0), t.stride(1), out.stride(0), out.stride(1), t.shape[1])
+        return RopeTensor(t.data_ptr(), out.data_ptr(), si[0], si[1], so[0], so[1], t.shape[1])
 
     def apply(self, positions, q, q_out, k=None, k_out=None, inverse=False):
         """q_out (and k_out) <- q (and k) [tokens, heads, d_head] turned by positions (int32 [tokens, axes], or None for
         the token's index) on the current stream; any token and head strides, out may be in itself."""
-        tokens = q.shape[0]
+        a = self._tensor(q, q_out)
+        tokens, _, d = q.shape
+        at = None
         if positions is not None:
             import torch
-            if positions.dtype != torch.int32 or tuple(positions.shape) != (tokens, self.n_axes) or not positions.is_contiguous():
+            if positions.shape != (tokens, self.n_axes) or positions.dtype != torch.int32 or not positions.is_contiguous():
                 raise ValueError(f"Rope: positions must be contiguous int32 [{tokens}, {self.n_axes}]")
-        a = self._tensor(q, q_out, q)
-        b = self._tensor(k, k_out, q) if k is not None else None
-        _on_device(positions, q, q_out, k, k_out)
-        check(lib().edb200_rope_apply(self.handle, C.byref(a), C.byref(b) if b is not None else None, torch_dtype_id(q),
-                                      q.shape[2], tokens, ptr(positions), int(inverse), current_stream()))
+            at = positions.data_ptr()
+        b = None
+        if k is not None:
+            if k.shape[0] != tokens or k.shape[2] != d or k.dtype != q.dtype:
+                raise ValueError("Rope: q and k share tokens, d_head and type")
+            b = C.byref(self._tensor(k, k_out))
+        st = lib().edb200_rope_apply(self.handle, C.byref(a), b, torch_dtype_id(q), d, tokens, at, 1 if inverse else 0,
+                                     _launch_stream(positions, q, q_out, k, k_out))
+        if st:
+            check(st)
 
     def __del__(self):
         if getattr(self, "handle", None) and _lib is not None:
