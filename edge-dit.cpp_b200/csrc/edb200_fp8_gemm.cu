@@ -21,7 +21,7 @@ namespace f8g {
 
 constexpr int BK = 128;                       // bytes = values of a k block
 constexpr uint32_t kFmtE4M3 = 0;              // kind::f8f6f4
-constexpr int PITCH = 36;                     // words between rows of an epilogue staging buffer (32 + 4: no conflicts)
+constexpr int SCALE_PITCH = 9;                // words between rows of eight scales in shared memory (no conflicts)
 
 struct Params {
     const float* xs;
@@ -63,24 +63,21 @@ __device__ __forceinline__ void mma_f8_ss_pair(uint32_t tmem_d, uint64_t adesc, 
         : "memory");
 }
 
-// acc[i] += s * r[i], two elements an instruction.  The packed form has the scalar one's rate (2.2 clocks for two) in half
-// the issue slots, and the slots matter more: eight warps of back-to-back scalar FMAs left the issuing warp none, and the
-// tensor pipe stood still until they were done.  Sums are held as register pairs throughout.
+// acc[i] += s * r[i], two elements an instruction: the packed form has the scalar one's rate (2.2 clocks for two) in half
+// the issue slots.  Those matter: eight warps of back-to-back scalar FMAs left the issuing warp none, and the tensor pipe
+// stood still until they were done.
 template <int N, int R>
-__device__ __forceinline__ void promote(uint64_t (&acc)[N], int at, const uint32_t (&r)[R], float s) {
+__device__ __forceinline__ void promote(float (&acc)[N], int at, const uint32_t (&r)[R], float s) {
     uint64_t ss;
     asm("mov.b64 %0, {%1, %1};" : "=l"(ss) : "f"(s));
 #pragma unroll
-    for (int i = 0; i < R / 2; ++i) {
-        uint64_t b;
-        asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "r"(r[2 * i]), "r"(r[2 * i + 1]));
-        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[at / 2 + i]) : "l"(b), "l"(ss));
+    for (int i = 0; i < R; i += 2) {
+        uint64_t a, b;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(acc[at + i]), "f"(acc[at + i + 1]));
+        asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "r"(r[i]), "r"(r[i + 1]));
+        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(b), "l"(ss));
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[at + i]), "=f"(acc[at + i + 1]) : "l"(a));
     }
-}
-template <int N>
-__device__ __forceinline__ void unpack_sums(const uint64_t (&sum)[N], float (&v)[2 * N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) asm("mov.b64 {%0, %1}, %2;" : "=f"(v[2 * i]), "=f"(v[2 * i + 1]) : "l"(sum[i]));
 }
 
 // The activations by exp and one division: gelu_tanh(v) = v / (1 + exp(-2 u)), exact to a few f32 roundings.
@@ -105,64 +102,80 @@ __device__ __forceinline__ void bias_act(float (&v)[N], const float* bias, int a
     }
 }
 
-// A warp's staged rows [32][32 words] to memory, `words` (16 or 32) of each row, 16 bytes a lane: whole 64- or 128-byte
-// runs of a row per store.  row0 / byte0: first row and first byte in a row of the staged piece; row_bytes: end of a row.
+// Epilogue of a pair's promotion warp: lane l holds row m_first + l, columns n0 .. n0 + N - 1 (biased, activated), and memory
+// wants runs of a row.  Pieces of 64 bytes a row go through the warp's staging buffer; then four lanes a row move 16 bytes
+// each, eight rows an instruction.
+constexpr int PITCH = 20;                     // words between staged rows (16 + 4: no conflicts)
+
+// Rows 8 i + lane / 4 of a staged piece, this lane's four words: put(row of the warp, quarter of the 64 bytes, words).
 template <typename F>
-__device__ __forceinline__ void copy_out(const float* stage, int words, int lane, const F& put) {
-    const int per = words / 4;               // lanes a row: 8 or 4
-    const int r0 = lane / per, c = (lane - r0 * per) * 4;
-    for (int r = r0; r < 32; r += 32 / per) put(r, c, *reinterpret_cast<const uint4*>(stage + r * PITCH + c));
+__device__ __forceinline__ void copy_out(const float* stage, int lane, const F& put) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + (lane >> 2);
+        put(i, r, *reinterpret_cast<const uint4*>(stage + r * PITCH + 4 * (lane & 3)));
+    }
 }
 
-// Epilogue of one thread's row m, columns n0 .. n0 + N - 1 (already biased and activated, in registers), through the
-// warp's staging buffer.  amax: of the row's 128 columns (e4m3 output).
+// amax: of the row's 128 columns (e4m3 output)
 template <int N>
 __device__ __forceinline__ void store_rows(const Params& P, const float (&v)[N], int m_first, int n0, int lane, float* stage,
                                            const float* gate, float amax) {
-    const bool inside = n0 + N <= P.N;
+    const int rows = P.M - m_first;           // of the warp's, inside
+    const int q = lane & 3;
     if (P.out_dtype == EDB200_TYPE_F32) {
+        const long long at = static_cast<long long>(m_first + (lane >> 2)) * P.ldo;
+        const long long res_at = static_cast<long long>(m_first + (lane >> 2)) * P.ld_res;
 #pragma unroll
-        for (int c = 0; c < N / 32; ++c) {
-            __syncwarp();
+        for (int c = 0; c < N / 16; ++c) {    // 16 columns a piece
+            const int n = n0 + 16 * c + 4 * q;
+            float4 res[4];
+            if (P.gate != nullptr) {          // on their way while the piece is staged
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-                *reinterpret_cast<float4*>(stage + lane * PITCH + i) = make_float4(v[32 * c + i], v[32 * c + i + 1], v[32 * c + i + 2], v[32 * c + i + 3]);
+                for (int i = 0; i < 4; ++i) {
+                    if (8 * i + (lane >> 2) < rows && n + 4 <= P.N) {
+                        res[i] = *reinterpret_cast<const float4*>(P.residual + res_at + 8 * i * P.ld_res + n);
+                    }
+                }
             }
             __syncwarp();
-            copy_out(stage, 32, lane, [&](int r, int col, uint4 u) {
-                const long long m = m_first + r;
-                const int n = n0 + 32 * c + col;
-                if (m >= P.M || n >= P.N) return;
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                *reinterpret_cast<float4*>(stage + lane * PITCH + i) = make_float4(v[16 * c + i], v[16 * c + i + 1], v[16 * c + i + 2], v[16 * c + i + 3]);
+            }
+            __syncwarp();
+            const float4 g = *reinterpret_cast<const float4*>(gate + 16 * c + 4 * q);
+            copy_out(stage, lane, [&](int i, int r, uint4 u) {
+                if (r >= rows || n >= P.N) return;
                 float4 x = *reinterpret_cast<float4*>(&u);
-                float* o = static_cast<float*>(P.out) + m * P.ldo + n;
-                if (inside || n + 4 <= P.N) {
+                float* o = static_cast<float*>(P.out) + at + 8 * i * P.ldo + n;
+                if (n + 4 <= P.N) {
                     if (P.gate != nullptr) {
-                        const float4 g = *reinterpret_cast<const float4*>(gate + 32 * c + col);
-                        const float4 q = *reinterpret_cast<const float4*>(P.residual + m * P.ld_res + n);
-                        x = make_float4(fmaf(g.x, x.x, q.x), fmaf(g.y, x.y, q.y), fmaf(g.z, x.z, q.z), fmaf(g.w, x.w, q.w));
+                        x = make_float4(fmaf(g.x, x.x, res[i].x), fmaf(g.y, x.y, res[i].y), fmaf(g.z, x.z, res[i].z), fmaf(g.w, x.w, res[i].w));
                     }
                     *reinterpret_cast<float4*>(o) = x;
-                } else {
-                    const float w[4] = {x.x, x.y, x.z, x.w};
-                    for (int e = 0; e < P.N - n; ++e) {
-                        float y = e == 0 ? w[0] : e == 1 ? w[1] : w[2];
-                        if (P.gate != nullptr) y = fmaf(gate[32 * c + col + e], y, P.residual[m * P.ld_res + n + e]);
-                        o[e] = y;
+                } else {                      // the last columns of a row that does not divide
+                    const float w[3] = {x.x, x.y, x.z}, h[3] = {g.x, g.y, g.z};
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) {
+                        if (n + e >= P.N) continue;
+                        o[e] = P.gate != nullptr ? fmaf(h[e], w[e], P.residual[res_at + 8 * i * P.ld_res + n + e]) : w[e];
                     }
                 }
             });
         }
     } else if (P.out_dtype != EDB200_TYPE_F8_E4M3) {
         const bool bf = P.out_dtype == EDB200_TYPE_BF16;
+        uint16_t* base = static_cast<uint16_t*>(P.out) + static_cast<long long>(m_first + (lane >> 2)) * P.ldo;
 #pragma unroll
-        for (int c = 0; c < N / 64; ++c) {
+        for (int c = 0; c < N / 32; ++c) {    // 32 columns a piece
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 64; i += 8) {
+            for (int i = 0; i < 32; i += 8) {
                 uint32_t w[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float a = v[64 * c + i + 2 * j], b = v[64 * c + i + 2 * j + 1];
+                    const float a = v[32 * c + i + 2 * j], b = v[32 * c + i + 2 * j + 1];
                     if (bf) {
                         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
                         w[j] = *reinterpret_cast<const uint32_t*>(&h);
@@ -174,12 +187,11 @@ __device__ __forceinline__ void store_rows(const Params& P, const float (&v)[N],
                 *reinterpret_cast<uint4*>(stage + lane * PITCH + i / 2) = make_uint4(w[0], w[1], w[2], w[3]);
             }
             __syncwarp();
-            copy_out(stage, 32, lane, [&](int r, int col, uint4 u) {
-                const long long m = m_first + r;
-                const int n = n0 + 64 * c + 2 * col;
-                if (m >= P.M || n >= P.N) return;
-                uint16_t* o = static_cast<uint16_t*>(P.out) + m * P.ldo + n;
-                if (inside || n + 8 <= P.N) {
+            const int n = n0 + 32 * c + 8 * q;
+            copy_out(stage, lane, [&](int i, int r, uint4 u) {
+                if (r >= rows || n >= P.N) return;
+                uint16_t* o = base + 8 * i * P.ldo + n;
+                if (n + 8 <= P.N) {
                     *reinterpret_cast<uint4*>(o) = u;
                 } else {
                     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -193,36 +205,37 @@ __device__ __forceinline__ void store_rows(const Params& P, const float (&v)[N],
     } else {
         float s, inv;
         f8_scale(amax, s, inv);
-        __syncwarp();
+        if (lane < rows && (n0 & 127) == 0 && n0 < P.N) P.out_scale[static_cast<long long>(m_first + lane) * P.ld_os + (n0 >> 7)] = s;
+        uint8_t* base = static_cast<uint8_t*>(P.out) + static_cast<long long>(m_first + (lane >> 2)) * P.ldo;
 #pragma unroll
-        for (int i = 0; i < N; i += 16) {
-            uint32_t w[4];
+        for (int c = 0; c < N / 64; ++c) {    // 64 columns a piece
+            __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                w[j] = f8_pack4(f8_scaled(v[i + 4 * j], inv), f8_scaled(v[i + 4 * j + 1], inv), f8_scaled(v[i + 4 * j + 2], inv),
-                                f8_scaled(v[i + 4 * j + 3], inv));
-            }
-            *reinterpret_cast<uint4*>(stage + lane * PITCH + i / 4) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        if (m_first + lane < P.M && (n0 & 127) == 0 && n0 < P.N) {
-            P.out_scale[static_cast<long long>(m_first + lane) * P.ld_os + (n0 >> 7)] = s;
-        }
-        __syncwarp();
-        copy_out(stage, N / 4, lane, [&](int r, int col, uint4 u) {
-            const long long m = m_first + r;
-            const int n = n0 + 4 * col;
-            if (m >= P.M || n >= P.N) return;
-            uint8_t* o = static_cast<uint8_t*>(P.out) + m * P.ldo + n;
-            if (inside || n + 16 <= P.N) {
-                *reinterpret_cast<uint4*>(o) = u;
-            } else {
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            for (int i = 64 * c; i < 64 * c + 64; i += 16) {
+                uint32_t w[4];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    if (n + e < P.N) o[e] = static_cast<uint8_t>(w[e >> 2] >> (8 * (e & 3)));
+                for (int j = 0; j < 4; ++j) {
+                    w[j] = f8_pack4(f8_scaled(v[i + 4 * j], inv), f8_scaled(v[i + 4 * j + 1], inv),
+                                    f8_scaled(v[i + 4 * j + 2], inv), f8_scaled(v[i + 4 * j + 3], inv));
                 }
+                *reinterpret_cast<uint4*>(stage + lane * PITCH + (i - 64 * c) / 4) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-        });
+            __syncwarp();
+            const int n = n0 + 64 * c + 16 * q;
+            copy_out(stage, lane, [&](int i, int r, uint4 u) {
+                if (r >= rows || n >= P.N) return;
+                uint8_t* o = base + 8 * i * P.ldo + n;
+                if (n + 16 <= P.N) {
+                    *reinterpret_cast<uint4*>(o) = u;
+                } else {
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        if (n + e < P.N) o[e] = static_cast<uint8_t>(w[e >> 2] >> (8 * (e & 3)));
+                    }
+                }
+            });
+        }
     }
 }
 
@@ -235,78 +248,201 @@ __device__ __forceinline__ float row_magnitude(const float (&v)[N], int n0, int 
     return a;
 }
 
+// Four neighbouring features of token m in each lane of a warp: the 128 columns of one e4m3 block.
+__device__ __forceinline__ void store_token(const Params& P, const float (&y)[4], long long m, int n, int lane) {
+    const bool whole = n + 4 <= P.N;
+    if (P.out_dtype == EDB200_TYPE_F8_E4M3) {
+        float a = row_magnitude(y, n, P.N);
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, k));
+        float s, inv;
+        f8_scale(a, s, inv);
+        const uint32_t w = f8_pack4(f8_scaled(y[0], inv), f8_scaled(y[1], inv), f8_scaled(y[2], inv), f8_scaled(y[3], inv));
+        uint8_t* o = static_cast<uint8_t*>(P.out) + m * P.ldo + n;
+        if (whole) {
+            *reinterpret_cast<uint32_t*>(o) = w;
+        } else {
+            for (int e = 0; e < P.N - n; ++e) o[e] = static_cast<uint8_t>(w >> (8 * e));
+        }
+        if (lane == 0) P.out_scale[m * P.ld_os + (n >> 7)] = s;
+        return;
+    }
+    if (P.out_dtype == EDB200_TYPE_F32) {
+        float* o = static_cast<float*>(P.out) + m * P.ldo + n;
+        const float* q = P.residual + m * P.ld_res + n;   // read with a gate only
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (P.gate != nullptr && n + e < P.N) ? fmaf(__ldg(P.gate + n + e), y[e], q[e]) : y[e];
+        if (whole) {
+            *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (n + e < P.N) o[e] = v[e];
+            }
+        }
+        return;
+    }
+    uint16_t h[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        h[e] = P.out_dtype == EDB200_TYPE_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(y[e])) : __half_as_ushort(__float2half_rn(y[e]));
+    }
+    uint16_t* o = static_cast<uint16_t*>(P.out) + m * P.ldo + n;
+    if (whole) {
+        *reinterpret_cast<uint2*>(o) = make_uint2(h[0] | (uint32_t(h[1]) << 16), h[2] | (uint32_t(h[3]) << 16));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (n + e < P.N) o[e] = h[e];
+        }
+    }
+}
+
+// The end of a tile shared by `parts` CTAs of a cluster: sums[token][128 features] lie in each one's shared memory; every
+// CTA finishes each parts-th token, a warp per token and four features a lane.
+__device__ __forceinline__ void finish_tokens(const Params& P, const float* sums, int pitch, int tokens, int m0, int n0, int part,
+                                              int parts, int warp, int warps, int lane, bool bad) {
+    if (parts > 1) {
+        cluster_sync_all();
+    } else {
+        __syncthreads();
+    }
+    const int n = n0 + 4 * lane;
+    float bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias[e] = (P.bias != nullptr && n + e < P.N) ? __ldg(P.bias + n + e) : 0.0f;
+    // two tokens at a time, and every part's sums asked for before the first is added: the reads' latency is the time here
+    const int stride = parts * warps;
+    for (int t0 = part + parts * warp; t0 < tokens && m0 + t0 < P.M; t0 += 2 * stride) {
+        float4 q[2][8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int t = t0 + i * stride < tokens ? t0 + i * stride : t0;
+            if (parts == 1) {
+                q[i][0] = *reinterpret_cast<const float4*>(sums + t * pitch + 4 * lane);
+            } else {
+#pragma unroll
+                for (int p = 0; p < 8; ++p) {
+                    if (p < parts) q[i][p] = cluster_load4(sums + t * pitch + 4 * lane, p);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int t = t0 + i * stride;
+            float4 v = q[i][0];
+#pragma unroll
+            for (int p = 1; p < 8; ++p) {
+                if (p < parts) v.x += q[i][p].x, v.y += q[i][p].y, v.z += q[i][p].z, v.w += q[i][p].w;
+            }
+            float y[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
+            if (P.act != EDB200_ACT_NONE) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = act_one(y[e], P.act);
+            }
+            if (t < tokens && m0 + t < P.M && !bad) store_token(P, y, m0 + t, n, lane);   // uniform over the warp
+        }
+    }
+    if (parts > 1) cluster_sync_all();   // no CTA leaves while another reads its sums
+}
+
+// One group of scales: xs of 128 rows from m0 on, this lane's block `at`, as [row][8 of SCALE_PITCH], then ws of `halves` weight blocks.
+// Four rows of eight blocks a load; rows past the end follow the last one.
+__device__ __forceinline__ void bring_scales(const Params& P, float* dst, int m0, int at, int n_block, int halves, int lane) {
+    const int nb_last = (P.N - 1) >> 7;
+    if (lane < 8 * halves) {
+        const int nb = n_block + (lane >> 3);
+        dst[128 * SCALE_PITCH + lane] = __ldg(P.ws + static_cast<long long>(nb < nb_last ? nb : nb_last) * P.ld_ws + at);
+    }
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        const int m = m0 + r < P.M ? m0 + r : P.M - 1;
+        dst[r * SCALE_PITCH + (lane & 7)] = __ldg(P.xs + m * P.ld_xs + at);
+    }
+}
+
 // ------------------------------------------------------------------ one CTA per 128 tokens x 128 features
+// For products whose 256 x 256 tiles are too few for the CTA pairs below.  Tokens in the lanes, features in the columns of
+// four accumulators; eight promotion warps of 32 tokens x 64 features, warp 2 bringing the scales as in the pairs.  Where
+// the tiles leave SMs idle a cluster of up to eight CTAs shares one, each a run of its k blocks; sums meet in shared memory
+// and are added in the order of the parts.
 namespace tile {
-constexpr int STAGES = 5;
+constexpr int STAGES = 5, BUFS = 4;
 constexpr int A_BYTES = 128 * BK, STAGE_BYTES = 2 * A_BYTES;
 constexpr int WARPS = 8;                                        // promotion warps
 constexpr int CPT = 64;                                         // columns of a promotion thread
-constexpr int OFF_STAGE = STAGES * STAGE_BYTES;
-constexpr int OFF_VEC = OFF_STAGE + WARPS * 32 * PITCH * 4;     // bias [128], gate [128], row maxima [2][128]
-constexpr int OFF_BAR = OFF_VEC + 512 * 4;
+constexpr int THREADS = 32 * (WARPS + 4);                       // warp 0 TMA, 1 MMA, 2 scales, 4-11 promotion; all store
+constexpr int SUM_PITCH = 132;                                  // words between rows of the sums (no conflicts)
+constexpr int SCALE_WORDS = 128 * SCALE_PITCH + 8;              // a group of eight blocks: [row][8], ws [8]
+constexpr int OFF_SCALE = STAGES * STAGE_BYTES;
+constexpr int OFF_BAR = OFF_SCALE + 2 * SCALE_WORDS * 4;
 constexpr int SMEM_BYTES = OFF_BAR + 256 + 1024;
-constexpr int THREADS = 32 * (WARPS + 2);
-static_assert(SMEM_BYTES <= 227 * 1024, "shared memory plan");
+static_assert(SMEM_BYTES <= 227 * 1024 && 128 * SUM_PITCH * 4 <= OFF_SCALE, "shared memory plan");
 }  // namespace tile
 
 __global__ void __launch_bounds__(tile::THREADS, 1)
 fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-                const __grid_constant__ Params P) {
+                const __grid_constant__ Params P, const int parts) {
     using namespace tile;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float* s_bias = reinterpret_cast<float*>(smem + OFF_VEC);
-    float* s_gate = s_bias + 128;
-    float* s_max = s_gate + 128;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + OFF_BAR);   // [STAGES]
     uint64_t* empty = full + STAGES;                                // [STAGES]
-    uint64_t* acc_full = empty + STAGES;                            // [2]
-    uint64_t* acc_empty = acc_full + 2;                             // [2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    uint64_t* acc_full = empty + STAGES;                            // [BUFS]
+    uint64_t* acc_empty = acc_full + BUFS;                          // [BUFS]
+    uint64_t* sc_full = acc_empty + BUFS;                           // [2]
+    uint64_t* sc_empty = sc_full + 2;                               // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* scales = reinterpret_cast<float*>(smem + OFF_SCALE);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n_tile = blockIdx.x / P.m_tiles, m_tile = blockIdx.x - n_tile * P.m_tiles;
+    const int t = blockIdx.x / parts, part = blockIdx.x - t * parts;   // a cluster is `parts` neighbours: its rank
+    const int n_tile = t / P.m_tiles, m_tile = t - n_tile * P.m_tiles;
     const int n0 = n_tile * 128, m0 = m_tile * 128;
+    const int b_first = static_cast<int>(static_cast<long long>(P.kblocks) * part / parts);
+    const int blocks = static_cast<int>(static_cast<long long>(P.kblocks) * (part + 1) / parts) - b_first;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < BUFS; ++i) {
             mbar_init(&acc_full[i], 1);
             mbar_init(&acc_empty[i], WARPS);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sc_full[i], 1);
+            mbar_init(&sc_empty[i], WARPS);
         }
         *abort_flag = 0;
         fence_mbar_init();
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, 256);
+        tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&map_x);
         tma_prefetch_desc(&map_w);
     }
-    if (warp >= 2) {
-        const int t = threadIdx.x - 64, n = n0 + (t & 127);
-        const float* src = t < 128 ? P.bias : P.gate;
-        s_bias[t] = (src != nullptr && n < P.N) ? __ldg(src + n) : 0.0f;   // s_gate follows s_bias
-    }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
+    float sum[CPT];
 
     if (warp == 0) {
         uint32_t s = 0, ph = 0;
-        for (int b = 0; b < P.kblocks; ++b) {
+        for (int b = 0; b < blocks; ++b) {
             if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, P.err)) break;
             if (elect_one()) {
                 uint8_t* stage = smem + s * STAGE_BYTES;
                 mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
-                tma_load_2d(stage, &map_x, &full[s], b * BK, m0);
-                tma_load_2d(stage + A_BYTES, &map_w, &full[s], b * BK, n0);
+                tma_load_2d(stage, &map_x, &full[s], (b_first + b) * BK, m0);
+                tma_load_2d(stage + A_BYTES, &map_w, &full[s], (b_first + b) * BK, n0);
             }
             __syncwarp();
             if (++s == STAGES) {
@@ -317,8 +453,8 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     } else if (warp == 1) {
         const uint32_t idesc = make_idesc(kDFmtF32, kFmtE4M3, kFmtE4M3, 0, 0, 128, 128);
         uint32_t s = 0, ph = 0;
-        for (int b = 0; b < P.kblocks; ++b) {
-            const uint32_t buf = b & 1, aph = (b >> 1) & 1;
+        for (int b = 0; b < blocks; ++b) {
+            const uint32_t buf = b % BUFS, aph = (b / BUFS) & 1u;
             if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag, P.err)) break;
             if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
             tc_fence_after_sync();
@@ -329,8 +465,8 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     mma_f8_ss(tmem_base + buf * 128, make_smem_desc_sw128(a_addr + j * 32, 16, 1024),
                               make_smem_desc_sw128(b_addr + j * 32, 16, 1024), idesc, j > 0 ? 1u : 0u);
                 }
-                mma_commit(&empty[s]);
                 mma_commit(&acc_full[buf]);
+                mma_commit(&empty[s]);
             }
             __syncwarp();
             if (++s == STAGES) {
@@ -338,57 +474,64 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 ph ^= 1u;
             }
         }
-    } else {
-        const int quarter = warp & 3, side = (warp - 2) >> 2;   // lanes of tensor memory, half of the columns
+    } else if (warp == 2) {
+        for (int b = 0; b < blocks; b += 8) {
+            const int g = b >> 3;
+            if (!__all_sync(0xffffffffu, mbar_wait(&sc_empty[g & 1], ((g >> 1) & 1) ^ 1u, abort_flag, P.err))) break;
+            const int at = b_first + (b + (lane & 7) < blocks ? b + (lane & 7) : blocks - 1);
+            bring_scales(P, scales + (g & 1) * SCALE_WORDS, m0, at, n_tile, 1, lane);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sc_full[g & 1]);
+        }
+    } else if (warp >= 4) {
+        const int quarter = warp & 3, side = (warp - 4) >> 2;   // lanes of tensor memory, half of the columns
         const int row = quarter * 32 + lane;
-        const int m = m0 + row < P.M ? m0 + row : P.M - 1;      // rows past the end follow the last one, store nothing
-        const float* xs = P.xs + m * P.ld_xs;
-        const float* ws = P.ws + n_tile * P.ld_ws;
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + side * CPT;
-        uint64_t sum[CPT / 2];
 #pragma unroll
-        for (int i = 0; i < CPT / 2; ++i) sum[i] = 0;
-        float scale = __ldg(xs) * __ldg(ws);
-        bool ok = true;
-        for (int b = 0; b < P.kblocks; ++b) {
-            const uint32_t buf = b & 1, aph = (b >> 1) & 1;
-            const int nb = b + 1 < P.kblocks ? b + 1 : b;
-            const float next = __ldg(xs + nb) * __ldg(ws + nb);
-            ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aph, abort_flag, P.err));
-            if (!ok) break;
+        for (int i = 0; i < CPT; ++i) sum[i] = 0.0f;
+        for (int b = 0; b < blocks; ++b) {
+            const uint32_t buf = b % BUFS, aph = (b / BUFS) & 1u;
+            const int g = b >> 3;
+            bool ok = true;
+            if ((b & 7) == 0) ok = mbar_wait(&sc_full[g & 1], (g >> 1) & 1, abort_flag, P.err);
+            ok = ok && mbar_wait(&acc_full[buf], aph, abort_flag, P.err);
+            if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after_sync();
             uint32_t r0[32], r1[32];
             tmem_ld_32x32b_x32(taddr + buf * 128, r0);
+            const float* sc = scales + (g & 1) * SCALE_WORDS;
+            const float scale = sc[row * SCALE_PITCH + (b & 7)] * sc[128 * SCALE_PITCH + (b & 7)];
+            tmem_wait_ld();
             tmem_ld_32x32b_x32(taddr + buf * 128 + 32, r1);
+            promote(sum, 0, r0, scale);
             tmem_wait_ld();
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[buf]);
-            promote(sum, 0, r0, scale);
+            if (lane == 0) {
+                mbar_arrive(&acc_empty[buf]);
+                if ((b & 7) == 7) mbar_arrive(&sc_empty[g & 1]);
+            }
             promote(sum, 32, r1, scale);
-            scale = next;
         }
-        const int nc = n0 + side * CPT;
-        float amax = 0.0f;
-        float acc[CPT];
-        unpack_sums(sum, acc);
-        if (ok) bias_act(acc, s_bias + side * CPT, P.act);
-        if (P.out_dtype == EDB200_TYPE_F8_E4M3) {   // uniform: the row's other half lies in the other warp group
-            s_max[side * 128 + row] = row_magnitude(acc, nc, P.N);
-            named_bar_sync(1, 32 * WARPS);
-            amax = fmaxf(s_max[row], s_max[128 + row]);
-        }
-        if (ok) store_rows(P, acc, m0 + quarter * 32, nc, lane, reinterpret_cast<float*>(smem + OFF_STAGE) + (warp - 2) * 32 * PITCH, s_gate + side * CPT, amax);
     }
     tc_fence_before_sync();
-    __syncthreads();
-    if (*abort_flag) {
+    __syncthreads();            // every block has been read: the copies and MMAs of this CTA are done
+    const bool bad = *abort_flag != 0;
+    if (bad) {
         for (int i = 0; i < 200; ++i) __nanosleep(1000);   // let copies and MMAs in flight land
         __syncthreads();
     }
+    float* sums = reinterpret_cast<float*>(smem);   // [128][SUM_PITCH]
+    if (warp >= 4) {
+        const float (&v)[CPT] = sum;
+        float* o = sums + ((warp & 3) * 32 + lane) * SUM_PITCH + ((warp - 4) >> 2) * CPT;
+#pragma unroll
+        for (int i = 0; i < CPT; i += 4) *reinterpret_cast<float4*>(o + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    }
+    finish_tokens(P, sums, SUM_PITCH, 128, m0, n0, part, parts, warp, THREADS / 32, lane, bad);
     if (warp == 1) {
         tc_fence_after_sync();
-        tmem_dealloc(tmem_base, 256);
+        tmem_dealloc(tmem_base, 512);
     }
 }
 
@@ -413,7 +556,7 @@ constexpr int WARPS = 8;
 constexpr int CPT = 128;
 constexpr int OFF_STAGE = STAGES * STAGE_BYTES;
 constexpr int OFF_VEC = OFF_STAGE + WARPS * 32 * PITCH * 4;     // [2 tiles][2 halves][bias 128, gate 128]
-constexpr int SCALE_WORDS = 128 * 9 + 16;                        // a group: [row][8 blocks + 1], then ws [half][8]
+constexpr int SCALE_WORDS = 128 * SCALE_PITCH + 16;              // a group: [row][8 blocks], then ws [half][8]
 constexpr int OFF_SCALE = OFF_VEC + 2 * 2 * 256 * 4;
 constexpr int OFF_BAR = OFF_SCALE + 2 * SCALE_WORDS * 4;
 constexpr int SMEM_BYTES = OFF_BAR + 256 + 1024;
@@ -499,65 +642,68 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             const bool n_ok = nc + row < P.N;
             const float bias_v = (P.bias != nullptr && n_ok) ? __ldg(P.bias + nc + row) : 0.0f;
             const float gate_v = (P.gate != nullptr && n_ok) ? __ldg(P.gate + nc + row) : 0.0f;
-            uint64_t sum[CPT / 2];
+            float sum[CPT];
 #pragma unroll
-            for (int i = 0; i < CPT / 2; ++i) sum[i] = 0;
+            for (int i = 0; i < CPT; ++i) sum[i] = 0.0f;
             // One block's reading runs into the next one's: the barrier of block b + 1 is looked at and its first columns
             // are under way before block b's last products are added.
-            ok = __all_sync(0xffffffffu, mbar_wait(&sc_full[sg & 1u], (sg >> 1) & 1u, abort_flag, P.err));
+            ok = mbar_wait(&sc_full[sg & 1u], (sg >> 1) & 1u, abort_flag, P.err) &&
+                 mbar_wait(&acc_full[2 * side + (g & 1u)], (g >> 1) & 1u, abort_flag, P.err);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const float* sc = scales + (sg & 1u) * SCALE_WORDS;
-            float scale = sc[row * 9] * sc[128 * 9 + side * 8];
+            float scale = sc[row * SCALE_PITCH] * sc[128 * SCALE_PITCH + side * 8];
             uint32_t r0[32], r1[32];
-            ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[2 * side + (g & 1u)], (g >> 1) & 1u, abort_flag, P.err));
-            if (!ok) break;
             tc_fence_after_sync();
             tmem_ld_32x32b_x32(taddr + (g & 1u) * 128, r0);
+            tmem_ld_32x32b_x32(taddr + (g & 1u) * 128 + 32, r1);
             for (int b = 0; b < P.kblocks; ++b, ++g) {
-                const uint32_t at = taddr + (g & 1u) * 128;
-                const uint32_t nbuf = (g + 1) & 1u, nph = ((g + 1) >> 1) & 1u;
+                const uint32_t at = taddr + (g & 1u) * 128, next = taddr + ((g + 1) & 1u) * 128;
                 const float s = scale;
+                const bool more = b + 1 < P.kblocks;
                 tmem_wait_ld();
-                tmem_ld_32x32b_x32(at + 32, r1);
                 promote(sum, 0, r0, s);
-                tmem_wait_ld();
                 tmem_ld_32x32b_x32(at + 64, r0);
                 promote(sum, 32, r1, s);
-                tmem_wait_ld();
                 tmem_ld_32x32b_x32(at + 96, r1);
-                const bool there = mbar_test(&acc_full[2 * side + nbuf], nph);
-                promote(sum, 64, r0, s);
-                if (((b + 1) & 7) == 0 || b + 1 == P.kblocks) {   // the group is read
+                const bool there = mbar_test(&acc_full[2 * side + ((g + 1) & 1u)], ((g + 1) >> 1) & 1u);
+                if (((b + 1) & 7) == 0 || !more) {   // the group of scales is read
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sc_empty[sg & 1u]);
                     ++sg;
                     sc = scales + (sg & 1u) * SCALE_WORDS;
-                    if (b + 1 < P.kblocks) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(&sc_full[sg & 1u], (sg >> 1) & 1u, abort_flag, P.err));
-                        if (!ok) break;
-                    }
+                    if (more) ok = __all_sync(0xffffffffu, mbar_wait(&sc_full[sg & 1u], (sg >> 1) & 1u, abort_flag, P.err));
                 }
-                scale = sc[row * 9 + ((b + 1) & 7)] * sc[128 * 9 + side * 8 + ((b + 1) & 7)];   // unused after the last block
+                const float sx = sc[row * SCALE_PITCH + ((b + 1) & 7)], sw = sc[128 * SCALE_PITCH + side * 8 + ((b + 1) & 7)];
                 tmem_wait_ld();
                 tc_fence_before_sync();
                 if (lane == 0) mbar_arrive_relaxed((g & 1u) ? free1 : free0);
-                if (b + 1 < P.kblocks) {
-                    if (!__all_sync(0xffffffffu, there)) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[2 * side + nbuf], nph, abort_flag, P.err));
-                        if (!ok) break;
-                    }
+                scale = sx * sw;                                  // unused after the last block
+                if (__all_sync(0xffffffffu, there) && more) {
                     tc_fence_after_sync();
-                    tmem_ld_32x32b_x32(taddr + nbuf * 128, r0);
+                    promote(sum, 64, r0, s);
+                    tmem_ld_32x32b_x32(next, r0);
+                    promote(sum, 96, r1, s);
+                    tmem_ld_32x32b_x32(next + 32, r1);
+                } else {
+                    promote(sum, 64, r0, s);
+                    promote(sum, 96, r1, s);
+                    if (more) {
+                        ok = ok && __all_sync(0xffffffffu, mbar_wait(&acc_full[2 * side + ((g + 1) & 1u)], ((g + 1) >> 1) & 1u, abort_flag, P.err));
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        tmem_ld_32x32b_x32(next, r0);
+                        tmem_ld_32x32b_x32(next + 32, r1);
+                    }
                 }
-                promote(sum, 96, r1, s);
+                if (!ok) break;
             }
             if (!ok) break;
             float* vec = reinterpret_cast<float*>(smem + OFF_VEC) + (parity * 2 + side) * 256;
             vec[row] = bias_v;
             vec[128 + row] = gate_v;
             named_bar_sync(1 + side, 128);
-            float acc[CPT];
-            unpack_sums(sum, acc);
+            float (&acc)[CPT] = sum;
             bias_act(acc, vec, P.act);
             float amax = 0.0f;
             if (P.out_dtype == EDB200_TYPE_F8_E4M3) amax = row_magnitude(acc, nc, P.N);
@@ -620,7 +766,6 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 }
             }
         } else if (warp == 3) {
-            const int nb_last = (P.N - 1) >> 7;
             float* dst0 = reinterpret_cast<float*>(smem + OFF_SCALE);
             uint32_t sg = 0;
             bool ok = true;
@@ -631,18 +776,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 for (int b = 0; b < P.kblocks; b += 8, ++sg) {
                     ok = __all_sync(0xffffffffu, mbar_wait(&sc_empty[sg & 1u], ((sg >> 1) & 1u) ^ 1u, abort_flag, P.err));
                     if (!ok) break;
-                    float* dst = dst0 + (sg & 1u) * SCALE_WORDS;
                     const int at = b + (lane & 7) < P.kblocks ? b + (lane & 7) : P.kblocks - 1;
-                    if (lane < 16) {
-                        const int nb = 2 * n_tile + (lane >> 3);
-                        dst[128 * 9 + lane] = __ldg(P.ws + static_cast<long long>(nb < nb_last ? nb : nb_last) * P.ld_ws + at);
-                    }
-#pragma unroll 8
-                    for (int i = 0; i < 32; ++i) {   // four rows of eight blocks a load; rows past the end follow the last one
-                        const int r = 4 * i + (lane >> 3);
-                        const int m = m0 + r < P.M ? m0 + r : P.M - 1;
-                        dst[r * 9 + (lane & 7)] = __ldg(P.xs + m * P.ld_xs + at);
-                    }
+                    bring_scales(P, dst0 + (sg & 1u) * SCALE_WORDS, m0, at, 2 * n_tile, 2, lane);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sc_full[sg & 1u]);
                 }
@@ -674,6 +809,196 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     }
 }
 
+// ----------------------------------------------------------- few rows: 128 features x NT tokens, k split over a cluster
+// Bound: HBM, the weights read once.  The roles are turned round: features lie in the 128 lanes of tensor memory, tokens in
+// its columns, so that a tile wastes nothing on tokens that are not there; a column's scale is then one number per token
+// and block, laid out by warp 2 for eight blocks at a time.  Two CTAs share an SM and keep 160 KB of weights under way
+// there.  Where the tiles alone leave SMs idle, a cluster of up to eight CTAs takes a tile, each a run of its k blocks; the
+// partial sums meet in shared memory and are added in the order of the parts.
+namespace few {
+constexpr int THREADS = 256;                 // warp 0 TMA, 1 MMA, 2 scales, 4-7 promotion; all add up and store
+constexpr int W_BYTES = 128 * BK;
+template <int NT>
+struct Plan {
+    static constexpr int STAGES = NT >= 64 ? 4 : 5;
+    static constexpr int STAGE_BYTES = W_BYTES + NT * BK;
+    static constexpr int OFF_SCALE = STAGES * STAGE_BYTES;          // [2 groups][8 blocks][NT + 4]
+    static constexpr int OFF_BAR = OFF_SCALE + 2 * 8 * (NT + 4) * 4;
+    static constexpr int SMEM_BYTES = OFF_BAR + 256 + 1024;
+    static constexpr int BUFS = 4;                                  // accumulators under way
+    static constexpr int TMEM_COLS = BUFS * NT;                     // 64, 128 or 256
+    static_assert(NT * 128 * 4 <= OFF_SCALE, "partial sums take the stages' place");
+    static_assert(SMEM_BYTES <= 113 * 1024, "two CTAs an SM");
+};
+}  // namespace few
+
+template <int NT>
+__global__ void __launch_bounds__(few::THREADS, 2)
+fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+               const __grid_constant__ Params P, const int parts) {
+    using namespace few;
+    using L = Plan<NT>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);   // [STAGES]
+    uint64_t* empty = full + L::STAGES;                                // [STAGES]
+    uint64_t* acc_full = empty + L::STAGES;                            // [BUFS]
+    uint64_t* acc_empty = acc_full + L::BUFS;                          // [BUFS]
+    uint64_t* sc_full = acc_empty + L::BUFS;                           // [2]
+    uint64_t* sc_empty = sc_full + 2;                                  // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* scales = reinterpret_cast<float*>(smem + L::OFF_SCALE);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tile = blockIdx.x / parts, part = blockIdx.x - tile * parts;   // a cluster is `parts` neighbours: its rank
+    const int n_tile = tile / P.m_tiles, m_tile = tile - n_tile * P.m_tiles;
+    const int n0 = n_tile * 128, m0 = m_tile * NT;
+    const int b_first = static_cast<int>(static_cast<long long>(P.kblocks) * part / parts);
+    const int blocks = static_cast<int>(static_cast<long long>(P.kblocks) * (part + 1) / parts) - b_first;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::STAGES; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < L::BUFS; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], 4);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sc_full[i], 1);
+            mbar_init(&sc_empty[i], 4);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, L::TMEM_COLS);
+        tmem_relinquish();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&map_x);
+        tma_prefetch_desc(&map_w);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    float acc[NT];
+
+    if (warp == 0) {
+        uint32_t s = 0, ph = 0;
+        for (int b = 0; b < blocks; ++b) {
+            if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, P.err)) break;
+            if (elect_one()) {
+                uint8_t* stage = smem + s * L::STAGE_BYTES;
+                mbar_arrive_expect_tx(&full[s], L::STAGE_BYTES);
+                tma_load_2d(stage, &map_w, &full[s], (b_first + b) * BK, n0);
+                tma_load_2d(stage + W_BYTES, &map_x, &full[s], (b_first + b) * BK, m0);
+            }
+            __syncwarp();
+            if (++s == L::STAGES) {
+                s = 0;
+                ph ^= 1u;
+            }
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc = make_idesc(kDFmtF32, kFmtE4M3, kFmtE4M3, 0, 0, 128, NT);
+        uint32_t s = 0, ph = 0;
+        for (int b = 0; b < blocks; ++b) {
+            const uint32_t buf = b % L::BUFS, aph = (b / L::BUFS) & 1u;
+            if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag, P.err)) break;
+            if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
+            tc_fence_after_sync();
+            if (elect_one()) {
+                const uint32_t a_addr = smem_u32(smem + s * L::STAGE_BYTES), b_addr = a_addr + W_BYTES;
+#pragma unroll
+                for (int j = 0; j < BK / 32; ++j) {
+                    mma_f8_ss(tmem_base + buf * NT, make_smem_desc_sw128(a_addr + j * 32, 16, 1024),
+                              make_smem_desc_sw128(b_addr + j * 32, 16, 1024), idesc, j > 0 ? 1u : 0u);
+                }
+                mma_commit(&acc_full[buf]);
+                mma_commit(&empty[s]);
+            }
+            __syncwarp();
+            if (++s == L::STAGES) {
+                s = 0;
+                ph ^= 1u;
+            }
+        }
+    } else if (warp == 2) {
+        const float* ws = P.ws + static_cast<long long>(n_tile) * P.ld_ws;
+        for (int b = 0; b < blocks; b += 8) {
+            const int g = b >> 3;
+            if (!__all_sync(0xffffffffu, mbar_wait(&sc_empty[g & 1], ((g >> 1) & 1) ^ 1u, abort_flag, P.err))) break;
+            float* dst = scales + (g & 1) * 8 * (NT + 4) + (lane & 7) * (NT + 4) + (lane >> 3);
+            const int at = b_first + (b + (lane & 7) < blocks ? b + (lane & 7) : blocks - 1);
+            const float w = __ldg(ws + at);
+#pragma unroll
+            for (int i = 0; i < NT / 4; ++i) {   // four tokens of eight blocks a load; tokens past the end follow the last
+                const int m = m0 + 4 * i + (lane >> 3) < P.M ? m0 + 4 * i + (lane >> 3) : P.M - 1;
+                dst[4 * i] = w * __ldg(P.xs + m * P.ld_xs + at);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sc_full[g & 1]);
+        }
+    } else if (warp >= 4) {
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[i] = 0.0f;
+        for (int b = 0; b < blocks; ++b) {
+            const uint32_t buf = b % L::BUFS, aph = (b / L::BUFS) & 1u;
+            const int g = b >> 3;
+            bool ok = true;
+            if ((b & 7) == 0) ok = mbar_wait(&sc_full[g & 1], (g >> 1) & 1, abort_flag, P.err);
+            ok = ok && mbar_wait(&acc_full[buf], aph, abort_flag, P.err);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_fence_after_sync();
+            const float* sc = scales + ((g & 1) * 8 + (b & 7)) * (NT + 4);
+#pragma unroll
+            for (int c = 0; c < NT; c += 16) {
+                uint32_t r[16];
+                tmem_ld_32x32b_x16(taddr + buf * NT + c, r);
+                float4 f[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[i] = *reinterpret_cast<const float4*>(sc + c + 4 * i);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    acc[c + 4 * i] = fmaf(__uint_as_float(r[4 * i]), f[i].x, acc[c + 4 * i]);
+                    acc[c + 4 * i + 1] = fmaf(__uint_as_float(r[4 * i + 1]), f[i].y, acc[c + 4 * i + 1]);
+                    acc[c + 4 * i + 2] = fmaf(__uint_as_float(r[4 * i + 2]), f[i].z, acc[c + 4 * i + 2]);
+                    acc[c + 4 * i + 3] = fmaf(__uint_as_float(r[4 * i + 3]), f[i].w, acc[c + 4 * i + 3]);
+                }
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&acc_empty[buf]);
+                if ((b & 7) == 7) mbar_arrive(&sc_empty[g & 1]);
+            }
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();            // every block has been read: the copies and MMAs of this CTA are done
+    const bool bad = *abort_flag != 0;
+    if (bad) {
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);   // let copies and MMAs in flight land
+        __syncthreads();
+    }
+    float* sums = reinterpret_cast<float*>(smem);   // [NT][128]
+    if (warp >= 4) {
+        const int f = (warp & 3) * 32 + lane;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sums[t * 128 + f] = acc[t];
+    }
+    finish_tokens(P, sums, 128, NT, m0, n0, part, parts, warp, THREADS / 32, lane, bad);
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, L::TMEM_COLS);
+    }
+}
+
 // Sets a kernel's dynamic shared memory once per device.
 template <typename K>
 static edb200_status_t allow_smem(K kern, int bytes, bool (&done)[64]) {
@@ -692,6 +1017,28 @@ static edb200_status_t operand_map(CUtensorMap* map, const void* base, int64_t k
                         CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Launches `tiles` clusters of `parts` CTAs.
+template <typename K>
+static edb200_status_t launch_parts(K kern, int64_t tiles, int parts, int threads, int smem, const CUtensorMap& map_x,
+                                    const CUtensorMap& map_w, const Params& P, cudaStream_t s) {
+    if (tiles * parts > 0x7fffffff) return fail(EDB200_ERR_UNSUPPORTED, "mul_mat_fp8: too many output tiles");
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * parts));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = static_cast<unsigned>(parts);
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    EDB_TRY(check_cuda(cudaLaunchKernelEx(&cfg, kern, map_x, map_w, P, parts), "mul_mat_fp8 launch"));
+    count_launch();
+    return EDB200_OK;
+}
+
 static edb200_status_t launch_tile(const edb200_fp8_weight_t& w, const void* x, int64_t m, int64_t ldx, Params& P, cudaStream_t s) {
     CUtensorMap map_x, map_w;
     EDB_TRY(operand_map(&map_x, x, w.k, m, ldx, 128));
@@ -700,10 +1047,24 @@ static edb200_status_t launch_tile(const edb200_fp8_weight_t& w, const void* x, 
     EDB_TRY(allow_smem(fp8_tile_kernel, tile::SMEM_BYTES, done));
     P.m_tiles = static_cast<int>((m + 127) / 128);
     const int64_t tiles = (int64_t)P.m_tiles * ((w.n + 127) / 128);
-    if (tiles > 0x7fffffff) return fail(EDB200_ERR_UNSUPPORTED, "mul_mat_fp8: too many output tiles");
-    fp8_tile_kernel<<<static_cast<unsigned>(tiles), tile::THREADS, tile::SMEM_BYTES, s>>>(map_x, map_w, P);
-    count_launch();
-    return check_cuda(cudaGetLastError(), "mul_mat_fp8 launch");
+    int parts = 1;   // of k: while every tile's cluster still gets SMs of its own, four blocks each at least
+    while (parts < 8 && tiles * parts * 2 <= sm_count() && P.kblocks >= parts * 8) parts *= 2;
+    return launch_parts(fp8_tile_kernel, tiles, parts, tile::THREADS, tile::SMEM_BYTES, map_x, map_w, P, s);
+}
+
+template <int NT>
+static edb200_status_t launch_few(const edb200_fp8_weight_t& w, const void* x, int64_t m, int64_t ldx, Params& P, cudaStream_t s) {
+    CUtensorMap map_x, map_w;
+    EDB_TRY(operand_map(&map_x, x, w.k, m, ldx, NT));
+    EDB_TRY(operand_map(&map_w, w.w, w.k, w.n, w.ldw, 128));
+    static bool done[64] = {false};
+    EDB_TRY(allow_smem(fp8_few_kernel<NT>, few::Plan<NT>::SMEM_BYTES, done));
+    P.m_tiles = static_cast<int>((m + NT - 1) / NT);
+    const int64_t tiles = (int64_t)P.m_tiles * ((w.n + 127) / 128);
+    // parts of k: as many as two CTAs an SM have room for, two blocks each at least
+    int parts = 1;
+    while (parts < 8 && tiles * parts * 2 <= 2 * sm_count() && P.kblocks >= parts * 4) parts *= 2;
+    return launch_parts(fp8_few_kernel<NT>, tiles, parts, few::THREADS, few::Plan<NT>::SMEM_BYTES, map_x, map_w, P, s);
 }
 
 static edb200_status_t launch_pair(const edb200_fp8_weight_t& w, const void* x, int64_t m, int64_t ldx, Params& P, cudaStream_t s) {
@@ -810,6 +1171,16 @@ extern "C" edb200_status_t edb200_mul_mat_fp8(const edb200_fp8_weight_t* w, cons
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof(s, PROF_GEMM, 2.0 * (double)m * (double)w->n * (double)w->k,
                    (double)w->n * (double)w->k + (double)m * (double)w->k + (double)m * (double)w->n * esz);
-    if (((m + 255) / 256) * ((w->n + 255) / 256) >= 37) return f8g::launch_pair(*w, x, m, ldx, P, s);
+    // Which kernel, by measured time (k 1536 and 5120, n 1536 to 13824):
+    //   up to 64 tokens, and where tiles of 128 tokens would be half empty (129 to 192): weight streaming.  2 x 5120 x 30720
+    //     29 us (tiles 50), 64 x 5120 x 5120 13.9 (14.6), 154 x 5120 x 5120 20.4 (22.4); 96 x 5120 x 5120 19.7 (15.5).
+    //   from 37 tiles of 256 x 256 on, half of what the GPU holds: CTA pairs.  512 x 4096 x 5120 (40 tiles) 25 us (tiles 36);
+    //     256 x 5120 x 5120 (20 tiles) 28 (22).
+    //   else tiles of 128 x 128.
+    if (m <= 16) return f8g::launch_few<16>(*w, x, m, ldx, P, s);
+    if (m <= 32) return f8g::launch_few<32>(*w, x, m, ldx, P, s);
+    const int64_t pairs = ((m + 255) / 256) * ((w->n + 255) / 256);
+    if (m <= 64 || (m > 128 && m <= 192 && pairs < 37)) return f8g::launch_few<64>(*w, x, m, ldx, P, s);
+    if (pairs >= 37) return f8g::launch_pair(*w, x, m, ldx, P, s);
     return f8g::launch_tile(*w, x, m, ldx, P, s);
 }

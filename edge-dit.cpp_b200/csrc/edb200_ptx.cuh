@@ -338,6 +338,16 @@ __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Four f32 from the shared memory of CTA `rank` of the cluster, at the place `p` has in this CTA's.
+__device__ __forceinline__ float4 cluster_load4(const float* p, uint32_t rank) {
+    uint32_t at;
+    float4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
 // Arrive on the barrier that sits at `bar`'s offset in the shared memory of cluster CTA 0 (the pair's leader).
 // Default (CTA-scope release) semantics: what crosses the pair behind this signal is tensor memory written by
 // tcgen05.st (completed by tcgen05.wait::st before the arrive) and shared memory written by TMA (complete
