@@ -102,6 +102,20 @@ __device__ __forceinline__ void bias_act(float (&v)[N], const float* bias, int a
     }
 }
 
+// Largest magnitude of a thread's columns n0 .. that lie inside N.
+template <int N>
+__device__ __forceinline__ float row_peak(const float (&v)[N], int n0, int n_end) {
+    float a = 0.0f;
+    if (n0 + N <= n_end) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) a = f8_peak(a, v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) a = n0 + i < n_end ? f8_peak(a, v[i]) : a;
+    }
+    return a;
+}
+
 // Epilogue of a pair's promotion warp: lane l holds row m_first + l, columns n0 .. n0 + N - 1 (biased, activated), and memory
 // wants runs of a row.  Pieces of 64 bytes a row go through the warp's staging buffer; then four lanes a row move 16 bytes
 // each, eight rows an instruction.
@@ -117,7 +131,7 @@ __device__ __forceinline__ void copy_out(const float* stage, int lane, const F& 
     }
 }
 
-// amax: of the row's 128 columns (e4m3 output)
+// amax: of the row's 128 columns, none of them infinite (e4m3 output)
 template <int N>
 __device__ __forceinline__ void store_rows(const Params& P, const float (&v)[N], int m_first, int n0, int lane, float* stage,
                                            const float* gate, float amax) {
@@ -215,8 +229,7 @@ __device__ __forceinline__ void store_rows(const Params& P, const float (&v)[N],
                 uint32_t w[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    w[j] = f8_pack4(f8_scaled(v[i + 4 * j], inv), f8_scaled(v[i + 4 * j + 1], inv),
-                                    f8_scaled(v[i + 4 * j + 2], inv), f8_scaled(v[i + 4 * j + 3], inv));
+                    w[j] = f8_pack4(v[i + 4 * j] * inv, v[i + 4 * j + 1] * inv, v[i + 4 * j + 2] * inv, v[i + 4 * j + 3] * inv);
                 }
                 *reinterpret_cast<uint4*>(stage + lane * PITCH + (i - 64 * c) / 4) = make_uint4(w[0], w[1], w[2], w[3]);
             }
@@ -239,25 +252,24 @@ __device__ __forceinline__ void store_rows(const Params& P, const float (&v)[N],
     }
 }
 
-// Largest magnitude of a thread's columns n0 .. that lie inside N.
-template <int N>
-__device__ __forceinline__ float row_magnitude(const float (&v)[N], int n0, int n_end) {
-    float a = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) a = fmaxf(a, n0 + i < n_end ? f8_magnitude(v[i]) : 0.0f);
-    return a;
-}
-
 // Four neighbouring features of token m in each lane of a warp: the 128 columns of one e4m3 block.
 __device__ __forceinline__ void store_token(const Params& P, const float (&y)[4], long long m, int n, int lane) {
     const bool whole = n + 4 <= P.N;
     if (P.out_dtype == EDB200_TYPE_F8_E4M3) {
-        float a = row_magnitude(y, n, P.N);
+        float v[4] = {y[0], y[1], y[2], y[3]};
+        float a = row_peak(v, n, P.N);
 #pragma unroll
         for (int k = 16; k > 0; k >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, k));
+        if (f8_has_infinity(a)) {   // uniform
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = f8_no_infinity(v[e]);
+            a = row_peak(v, n, P.N);
+#pragma unroll
+            for (int k = 16; k > 0; k >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, k));
+        }
         float s, inv;
         f8_scale(a, s, inv);
-        const uint32_t w = f8_pack4(f8_scaled(y[0], inv), f8_scaled(y[1], inv), f8_scaled(y[2], inv), f8_scaled(y[3], inv));
+        const uint32_t w = f8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
         uint8_t* o = static_cast<uint8_t*>(P.out) + m * P.ldo + n;
         if (whole) {
             *reinterpret_cast<uint32_t*>(o) = w;
@@ -706,7 +718,14 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             float (&acc)[CPT] = sum;
             bias_act(acc, vec, P.act);
             float amax = 0.0f;
-            if (P.out_dtype == EDB200_TYPE_F8_E4M3) amax = row_magnitude(acc, nc, P.N);
+            if (P.out_dtype == EDB200_TYPE_F8_E4M3) {
+                amax = row_peak(acc, nc, P.N);
+                if (f8_has_infinity(amax)) {
+#pragma unroll
+                    for (int i = 0; i < CPT; ++i) acc[i] = f8_no_infinity(acc[i]);
+                    amax = row_peak(acc, nc, P.N);
+                }
+            }
             store_rows(P, acc, m_first, nc, lane, stage, vec + 128, amax);
         }
     } else {

@@ -13,23 +13,19 @@ namespace f8q {
 
 constexpr int THREADS = 256;
 
-// The 16 values lane l of a group holds of one row's block: columns c0 + 64 j + 8 l + e.
+// The 16 values lane l of a group holds of one row's block: columns c0 + 64 j + 8 l + e.  Columns from k on and rows that
+// are not there read zero.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load16(const T* row, int c0, int l, int k, bool live, float (&v)[16]) {
+    if (VEC && live && c0 + 128 <= k) {
+        load8(row + c0 + 8 * l, reinterpret_cast<float(&)[8]>(v[0]));
+        load8(row + c0 + 64 + 8 * l, reinterpret_cast<float(&)[8]>(v[8]));
+    } else {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int c = c0 + 64 * j + 8 * l;
-        float w[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (VEC && live && c + 8 <= k) {
-            load8(row + c, w);
-        } else if (live) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (c + e < k) w[e] = widen<T>(row[c + e]);
-            }
+        for (int i = 0; i < 16; ++i) {
+            const int c = c0 + 64 * (i >> 3) + 8 * l + (i & 7);
+            v[i] = live && c < k ? widen<T>(row[c]) : 0.0f;
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[8 * j + e] = w[e];
     }
 }
 
@@ -38,10 +34,9 @@ __device__ __forceinline__ void store16(uint8_t* row, int c0, int l, int k, cons
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int c = c0 + 64 * j + 8 * l;
-        if (c >= k) continue;
         float w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = f8_scaled(v[8 * j + e], inv);
+        for (int e = 0; e < 8; ++e) w[e] = __fmul_rn(v[8 * j + e], inv);
         const uint32_t lo = f8_pack4(w[0], w[1], w[2], w[3]), hi = f8_pack4(w[4], w[5], w[6], w[7]);
         if (VEC && c + 8 <= k) {
             *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
@@ -54,10 +49,19 @@ __device__ __forceinline__ void store16(uint8_t* row, int c0, int l, int k, cons
     }
 }
 
-__device__ __forceinline__ float magnitude16(const float (&v)[16]) {
+__device__ __forceinline__ float peak16(const float (&v)[16]) {
     float a = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) a = fmaxf(a, f8_magnitude(v[i]));
+    for (int i = 0; i < 16; ++i) a = f8_peak(a, v[i]);
+    return a;
+}
+__device__ __forceinline__ void no_infinities16(float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = f8_no_infinity(v[i]);
+}
+__device__ __forceinline__ float group_max(float a) {
+#pragma unroll
+    for (int m = 4; m > 0; m >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, m));
     return a;
 }
 
@@ -73,40 +77,57 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int k, 
     const bool live = static_cast<int64_t>(row) < rows;
     float v[16];
     load16<T, VEC>(x + static_cast<int64_t>(row) * ldx, b * 128, l, k, live, v);
-    float a = magnitude16(v);
-#pragma unroll
-    for (int m = 4; m > 0; m >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, m));
-    if (!live) return;
+    float a = group_max(peak16(v));
+    uint8_t* qr = q + static_cast<int64_t>(row) * ldq;
+    if (__any_sync(0xffffffffu, f8_has_infinity(a))) {   // some block of the warp holds an infinity
+        no_infinities16(v);
+        a = group_max(peak16(v));
+    }
     float s, inv;
     f8_scale(a, s, inv);
-    store16<VEC>(q + static_cast<int64_t>(row) * ldq, b * 128, l, k, v, inv);
-    if (l == 0) scale[static_cast<int64_t>(row) * ld_scale + b] = s;
+    if (live) store16<VEC>(qr, b * 128, l, k, v, inv);
+    if (live && l == 0) scale[static_cast<int64_t>(row) * ld_scale + b] = s;
 }
 
-// 128 x 128: a CTA per block, 32 rows at a time, all 64 values of a thread in registers.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(THREADS)
-quantize_tiles_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int k, uint8_t* __restrict__ q, int64_t ldq,
-                      float* __restrict__ scale, int64_t ld_scale) {
-    __shared__ float sh[THREADS / 32];
-    const int l = threadIdx.x & 7;
-    const int64_t row0 = static_cast<int64_t>(blockIdx.y) * 128 + (threadIdx.x >> 3);
-    const int c0 = blockIdx.x * 128;
-    float v[4][16];
-    float a = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t row = row0 + 32 * i;
-        load16<T, VEC>(x + row * ldx, c0, l, k, row < rows, v[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a = fmaxf(a, magnitude16(v[i]));
+template <int N>
+__device__ __forceinline__ float cta_max(float a, float* sh) {
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, m));
     if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) a = fmaxf(a, sh[i]);
+    for (int i = 0; i < N; ++i) a = fmaxf(a, sh[i]);
+    return a;
+}
+
+// 128 x 128: a CTA per block, 32 rows at a time, all 64 values of a thread in registers.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(THREADS, 3)
+quantize_tiles_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int k, uint8_t* __restrict__ q, int64_t ldq,
+                      float* __restrict__ scale, int64_t ld_scale) {
+    __shared__ float sh[2][THREADS / 32];
+    const int l = threadIdx.x & 7;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.y) * 128 + (threadIdx.x >> 3);
+    const int c0 = blockIdx.x * 128;
+    float v[4][16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t row = row0 + 32 * i;
+        load16<T, VEC>(x + row * ldx, c0, l, k, row < rows, v[i]);
+    }
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a = fmaxf(a, peak16(v[i]));
+    a = cta_max<THREADS / 32>(a, sh[0]);
+    if (f8_has_infinity(a)) {   // the same in every thread
+        a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            no_infinities16(v[i]);
+            a = fmaxf(a, peak16(v[i]));
+        }
+        a = cta_max<THREADS / 32>(a, sh[1]);
+    }
     float s, inv;
     f8_scale(a, s, inv);
 #pragma unroll

@@ -401,8 +401,8 @@ EDB200_API edb200_status_t edb200_mul_mat_fp8(const edb200_fp8_weight_t* w, cons
  *   or single tokens with 1; rows_per_mod 0: one row for all.  NULL: 1, 0, 0.
  *   z_dtype EDB200_TYPE_F8_E4M3: z is quantised as edb200_quantize_fp8 does with block_rows 1, scales to
  *   z_scale [rows, ld_z_scale].
- * y may alias residual or x where type and stride agree.  h up to 16384, any strides; rows of 16-byte aligned
- * addresses and strides with h a multiple of 8 take wide loads.  Generalises edb200_layernorm_modulate and
+ * y may alias residual or x where type and stride agree.  h up to 16384, any strides; with h a multiple of four and
+ * every row of every buffer aligned to four of its elements, wide accesses.  Generalises edb200_layernorm_modulate and
  * edb200_fused_residual_gate, which keep the reference's order of operations bit for bit; this one does not. */
 enum { EDB200_NORM_NONE = 0, EDB200_NORM_LAYER = 1, EDB200_NORM_RMS = 2 };
 typedef struct {
