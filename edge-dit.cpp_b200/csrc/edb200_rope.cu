@@ -42,6 +42,7 @@ struct Params {
     int n_axes, pairs, d_head, tokens_per_cta;
     int units_head;             // pieces of a head: turned ones first, then those that pass through
     int units_turned;
+    uint32_t inv_token, inv_head;   // 2^32 / (pieces of a token, of a head), rounded up
     float mul;
     float sign;                 // -1 turns back
     double turns[128];
@@ -79,6 +80,87 @@ __device__ __forceinline__ void store_piece(T* p, const float (&v)[W]) {
     }
 }
 
+// n / d by the product with 2^32 / d rounded up: exact while n d < 2^32, which the host sees to.
+__device__ __forceinline__ int divided(int n, uint32_t inverse, int d) { return d == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), inverse)); }
+
+template <int N>
+__device__ __forceinline__ void table(const float* p, float (&v)[N]) {   // N consecutive entries at a multiple of N
+    if constexpr (N >= 4) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(p + i);
+            v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+        }
+    } else if constexpr (N == 2) {
+        const float2 f = *reinterpret_cast<const float2*>(p);
+        v[0] = f.x, v[1] = f.y;
+    } else {
+        v[0] = *p;
+    }
+}
+
+// One piece on its way: where it comes from and goes to, its values.
+template <typename T, int W, bool HALF>
+struct Unit {
+    static constexpr int N = HALF ? W : (W == 1 ? 1 : W / 2);   // pairs
+    static constexpr bool TWO = HALF || W == 1;                 // a pair's members come from two places
+    const T* in;
+    T* out;
+    int pair, at_a, at_b;   // pair < 0: passes through
+    float a[W], b[TWO ? W : 1];
+
+    __device__ __forceinline__ void find(const Params& P, long long t0, int i, int per_token, int heads0) {
+        const int t = divided(i, P.inv_token, per_token);
+        const int r = i - t * per_token;
+        int head = divided(r, P.inv_head, P.units_head);
+        const int u = r - head * P.units_head;
+        const Tensor& x = P.t[head >= heads0 ? 1 : 0];
+        if (head >= heads0) head -= heads0;
+        in = static_cast<const T*>(x.in) + (t0 + t) * x.in_token + head * x.in_head;
+        out = static_cast<T*>(x.out) + (t0 + t) * x.out_token + head * x.out_head;
+        if (u < P.units_turned) {
+            const int p = u * N;
+            pair = t * P.pairs + p;
+            at_a = HALF ? p : 2 * p;
+            at_b = HALF ? p + P.pairs : 2 * p + 1;
+        } else {
+            pair = -1;
+            at_a = 2 * P.pairs + (u - P.units_turned) * W;
+        }
+    }
+    __device__ __forceinline__ void load() {
+        if (pair < 0 && in == out) return;   // in place already
+        load_piece<T, W>(in + at_a, a);
+        if (TWO && pair >= 0) load_piece<T, W>(in + at_b, reinterpret_cast<float(&)[W]>(b[0]));
+    }
+    __device__ __forceinline__ void turn(const float* cs, const float* sn) {
+        if (pair < 0) {
+            if (in != out) store_piece<T, W>(out + at_a, a);
+            return;
+        }
+        float c[N], s[N], ya[W];
+        table<N>(cs + pair, c);
+        table<N>(sn + pair, s);
+        if constexpr (TWO) {
+            float yb[W];
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                ya[e] = fmaf(a[e], c[e], -__fmul_rn(b[e], s[e]));
+                yb[e] = fmaf(a[e], s[e], __fmul_rn(b[e], c[e]));
+            }
+            store_piece<T, W>(out + at_a, ya);
+            store_piece<T, W>(out + at_b, yb);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                ya[2 * e] = fmaf(a[2 * e], c[e], -__fmul_rn(a[2 * e + 1], s[e]));
+                ya[2 * e + 1] = fmaf(a[2 * e], s[e], __fmul_rn(a[2 * e + 1], c[e]));
+            }
+            store_piece<T, W>(out + at_a, ya);
+        }
+    }
+};
+
 // W: values of a piece (16 bytes' worth, or 1).  A turned unit of the halves layout is two pieces, half a turned width
 // apart; of the interleaved layout W values (one pair of single values where W is 1).
 template <typename T, int W, bool HALF>
@@ -98,52 +180,15 @@ rope_kernel(const __grid_constant__ Params P) {
         cs[i] = c * P.mul;
         sn[i] = s * P.mul * P.sign;
     }
-    __syncthreads();
-    const int heads0 = P.t[0].heads, heads = heads0 + P.t[1].heads;
-    const int per_token = heads * P.units_head;
+    const int heads0 = P.t[0].heads;
+    const int per_token = (heads0 + P.t[1].heads) * P.units_head;
     const int total = nt * per_token;
+    __syncthreads();
     for (int i = threadIdx.x; i < total; i += THREADS) {
-        const int t = i / per_token;
-        int r = i - t * per_token;
-        int head = r / P.units_head;
-        const int u = r - head * P.units_head;
-        const Tensor& x = P.t[head >= heads0 ? 1 : 0];
-        if (head >= heads0) head -= heads0;
-        const T* in = static_cast<const T*>(x.in) + (t0 + t) * x.in_token + head * x.in_head;
-        T* out = static_cast<T*>(x.out) + (t0 + t) * x.out_token + head * x.out_head;
-        const float* c = cs + t * P.pairs;
-        const float* s = sn + t * P.pairs;
-        if (u >= P.units_turned) {   // channels beyond the spans
-            if (in != out) {
-                const int at = 2 * P.pairs + (u - P.units_turned) * W;
-                float v[W];
-                load_piece<T, W>(in + at, v);
-                store_piece<T, W>(out + at, v);
-            }
-        } else if (HALF || W == 1) {
-            const int p = u * W;
-            const int ia = HALF ? p : 2 * p, ib = HALF ? p + P.pairs : 2 * p + 1;
-            float a[W], b[W], ya[W], yb[W];
-            load_piece<T, W>(in + ia, a);
-            load_piece<T, W>(in + ib, b);
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                ya[e] = a[e] * c[p + e] - b[e] * s[p + e];
-                yb[e] = a[e] * s[p + e] + b[e] * c[p + e];
-            }
-            store_piece<T, W>(out + ia, ya);
-            store_piece<T, W>(out + ib, yb);
-        } else {
-            const int p = u * (W / 2);
-            float v[W], y[W];
-            load_piece<T, W>(in + 2 * p, v);
-#pragma unroll
-            for (int e = 0; e < W / 2; ++e) {
-                y[2 * e] = v[2 * e] * c[p + e] - v[2 * e + 1] * s[p + e];
-                y[2 * e + 1] = v[2 * e] * s[p + e] + v[2 * e + 1] * c[p + e];
-            }
-            store_piece<T, W>(out + 2 * p, y);
-        }
+        Unit<T, W, HALF> u;
+        u.find(P, t0, i, per_token, heads0);
+        u.load();
+        u.turn(cs, sn);
     }
 }
 
@@ -287,12 +332,17 @@ edb200_status_t edb200_rope_apply(const edb200_rope_t* r, const edb200_rope_tens
     const int piece = vec ? w : 1;
     P.units_turned = r->layout == EDB200_ROPE_HALF || piece == 1 ? r->pairs / piece : 2 * r->pairs / piece;
     P.units_head = P.units_turned + (d_head - 2 * r->pairs) / piece;
-    // tokens of a CTA: about eight pieces for each thread, their table within shared memory
+    // tokens of a CTA: about eight pieces for each thread, their table within shared memory, and two CTAs an SM before more
     const long long per_token = (long long)(P.t[0].heads + P.t[1].heads) * P.units_head;
-    if (per_token > 0x3fffffff) return fail(EDB200_ERR_UNSUPPORTED, "rope_apply: a token's heads hold too many channels");
     long long nt = 8 * rope::THREADS / per_token;
     if (nt > rope::TABLE / r->pairs) nt = rope::TABLE / r->pairs;
+    const long long even = (tokens + 2 * sm_count() - 1) / (2 * sm_count());
+    if (nt > even) nt = even;
     if (nt < 1) nt = 1;
+    // the kernel divides by products: pieces of a CTA times pieces of a token stay below 2^32
+    if (per_token >= 65536) return fail(EDB200_ERR_UNSUPPORTED, "rope_apply: a token's heads hold more than 65535 pieces");
+    P.inv_token = static_cast<uint32_t>((0x100000000ull + per_token - 1) / per_token);
+    P.inv_head = static_cast<uint32_t>((0x100000000ull + P.units_head - 1) / P.units_head);
     P.tokens_per_cta = static_cast<int>(nt);
     const long long grid = (tokens + nt - 1) / nt;
     if (grid > 0x7fffffff) return fail(EDB200_ERR_UNSUPPORTED, "rope_apply: too many tokens for one launch");

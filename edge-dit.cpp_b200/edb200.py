@@ -423,15 +423,25 @@ def mul_mat_q(w: QWeight, x, ep: Epilogue):
                                  current_stream()))
 
 
-def _launch_stream(*tensors):
-    """The current stream, as the C entries take it.  Every tensor must lie on the current device: the library
+_here = None     # () -> the current device; set with _raw_stream on first use (torch is imported then)
+_raw_stream = None
+
+
+def _launch_stream(tensors):
+    """The current stream, as the C entries take it.  Every tensor (or None) must lie on the current device: the library
     launches there."""
-    import torch
-    here = torch.cuda.current_device()
+    global _here, _raw_stream
+    if _here is None:
+        import torch
+        # the raw handle without a Stream object around it, where this torch has it: 1.2 us less a call
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda device: torch.cuda.current_stream(device).cuda_stream)
+        _here = torch.cuda.current_device
+    here = _here()
     for t in tensors:
         if t is not None and t.get_device() != here:
             raise ValueError(f"tensor on {t.device}, current device is cuda:{here}")
-    return torch.cuda.current_stream(here).cuda_stream
+    return _raw_stream(here)
 
 
 def _rows_of(t, what):
@@ -456,7 +466,7 @@ def quantize_fp8(x, q, scale, block_rows=1):
         raise ValueError("quantize_fp8: q must be float8_e4m3fn of x's shape")
     lds = _scale_rows(scale, -(-rows // block_rows), -(-k // 128), "quantize_fp8: scale")
     st = lib().edb200_quantize_fp8(x.data_ptr(), torch_dtype_id(x), _rows_of(x, "x"), rows, k, block_rows, q.data_ptr(),
-                                   _rows_of(q, "q"), scale.data_ptr(), lds, _launch_stream(x, q, scale))
+                                   _rows_of(q, "q"), scale.data_ptr(), lds, _launch_stream((x, q, scale)))
     if st:
         check(st)
 
@@ -484,7 +494,7 @@ def mul_mat_fp8(w: Fp8Weight, x, x_scale, ep: Epilogue, out_scale=None):
     ldos = _scale_rows(out_scale, m, -(-w.n // 128), "mul_mat_fp8: out_scale") if out_scale is not None else 0
     st = lib().edb200_mul_mat_fp8(w.ref, x.data_ptr(), x_scale.data_ptr(), m, _rows_of(x, "x"), ldxs, C.byref(ep),
                                   out_scale.data_ptr() if out_scale is not None else None, ldos,
-                                  _launch_stream(x, x_scale, w.w, w.scale, out_scale))
+                                  _launch_stream((x, x_scale, w.w, w.scale, out_scale)))
     if st:
         check(st)
 
@@ -497,47 +507,62 @@ def block_norm(residual, y=None, z=None, z_scale=None, x=None, gate=None, residu
     row for each rows_per_mod rows (0: one for all); z_scale with a float8_e4m3fn z."""
     shape = residual.shape
     rows, h = shape
-    px = py = pz = pzs = None
-    ldx = ldy = ldz = ldzs = x_id = z_id = 0
     stream_id = torch_dtype_id(residual)
+    px = py = pz = pzs = pg = psc = psh = None
+    ldx = ldy = ldz = ldzs = ld_mod = x_id = z_id = 0
     if x is not None:
+        if x.shape != shape:
+            raise ValueError("block_norm: x must have residual's shape")
         px, ldx, x_id = x.data_ptr(), _rows_of(x, "x"), torch_dtype_id(x)
     if y is not None:
+        if y.shape != shape or y.dtype != residual.dtype:
+            raise ValueError("block_norm: y must have residual's shape and type")
         py, ldy = y.data_ptr(), _rows_of(y, "y")
-        if y.dtype != residual.dtype:
-            raise ValueError("block_norm: y must have residual's type")
     if z is not None:
+        if z.shape != shape:
+            raise ValueError("block_norm: z must have residual's shape")
         pz, ldz, z_id = z.data_ptr(), _rows_of(z, "z"), torch_dtype_id(z)
-    if (x is not None and x.shape != shape) or (y is not None and y.shape != shape) or (z is not None and z.shape != shape):
-        raise ValueError("block_norm: x, y and z must have residual's shape")
     if z_scale is not None:
         pzs, ldzs = z_scale.data_ptr(), _scale_rows(z_scale, rows, -(-h // 128), "block_norm: z_scale")
     groups = -(-rows // rows_per_mod) if rows_per_mod else 1
-    ld, mod = 0, [None, None, None]
-    for i, t in enumerate((gate, scale, shift)):
-        if t is None:
-            continue
-        if t.dim() == 1:
-            t = t[None]
-        if t.shape[1] != h or t.shape[0] < groups or torch_dtype_id(t) != TYPE_F32:
-            raise ValueError(f"block_norm: gate, scale and shift must be float32 [{groups}, {h}]")
-        at = _rows_of(t, "modulation")
-        if groups > 1 and ld and at != ld:
-            raise ValueError("block_norm: gate, scale and shift must share one row stride")
-        ld, mod[i] = at, t.data_ptr()
-    affine = [None, None, None, None]
-    for i, t in enumerate((post_weight, post_bias, pre_weight, pre_bias)):
-        if t is not None:
-            if t.shape != (h,) or torch_dtype_id(t) != TYPE_F32 or not t.is_contiguous():
-                raise ValueError(f"block_norm: weights and biases must be contiguous float32 [{h}]")
-            affine[i] = t.data_ptr()
+    if gate is not None:
+        pg, ld_mod = _modulation(gate, groups, h, 0)
+    if scale is not None:
+        psc, ld_mod = _modulation(scale, groups, h, ld_mod)
+    if shift is not None:
+        psh, ld_mod = _modulation(shift, groups, h, ld_mod)
     d = BlockNormDesc(rows, h, px, ldx, residual.data_ptr(), _rows_of(residual, "residual"), py, ldy, pz, ldz, pzs, ldzs,
-                      *mod, ld, rows_per_mod, *affine, residual_scale, post_eps, pre_eps, x_id, stream_id, z_id, post_norm,
-                      pre_norm)
-    st = lib().edb200_block_norm(C.byref(d), _launch_stream(residual, x, y, z, z_scale, gate, scale, shift, post_weight,
-                                                            post_bias, pre_weight, pre_bias))
+                      pg, psc, psh, ld_mod, rows_per_mod, _affine(post_weight, h), _affine(post_bias, h),
+                      _affine(pre_weight, h), _affine(pre_bias, h), residual_scale, post_eps, pre_eps, x_id, stream_id,
+                      z_id, post_norm, pre_norm)
+    st = lib().edb200_block_norm(C.byref(d), _launch_stream((residual, x, y, z, z_scale, gate, scale, shift, post_weight,
+                                                             post_bias, pre_weight, pre_bias)))
     if st:
         check(st)
+
+
+def _modulation(t, groups, h, ld):
+    """Address and row stride of `groups` float32 rows of h values, which share one stride."""
+    shape = t.shape
+    if len(shape) == 1 and groups == 1 and shape[0] == h:
+        at = h
+    elif len(shape) == 2 and shape[1] == h and shape[0] >= groups:
+        at = _rows_of(t, "modulation")
+    else:
+        raise ValueError(f"block_norm: gate, scale and shift must be float32 [{groups}, {h}]")
+    if torch_dtype_id(t) != TYPE_F32 or (len(shape) == 1 and not t.is_contiguous()):
+        raise ValueError(f"block_norm: gate, scale and shift must be float32 [{groups}, {h}]")
+    if groups > 1 and ld and at != ld:
+        raise ValueError("block_norm: gate, scale and shift must share one row stride")
+    return t.data_ptr(), at
+
+
+def _affine(t, h):
+    if t is None:
+        return None
+    if t.shape != (h,) or torch_dtype_id(t) != TYPE_F32 or not t.is_contiguous():
+        raise ValueError(f"block_norm: weights and biases must be contiguous float32 [{h}]")
+    return t.data_ptr()
 
 
 class Rope:
@@ -580,7 +605,7 @@ class Rope:
                 raise ValueError("Rope: q and k share tokens, d_head and type")
             b = C.byref(self._tensor(k, k_out))
         st = lib().edb200_rope_apply(self.handle, C.byref(a), b, torch_dtype_id(q), d, tokens, at, 1 if inverse else 0,
-                                     _launch_stream(positions, q, q_out, k, k_out))
+                                     _launch_stream((positions, q, q_out, k, k_out)))
         if st:
             check(st)
 
