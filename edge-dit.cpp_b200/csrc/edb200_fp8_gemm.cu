@@ -252,24 +252,27 @@ __device__ __forceinline__ void store_rows(const Params& P, const float (&v)[N],
     }
 }
 
-// Four neighbouring features of token m in each lane of a warp: the 128 columns of one e4m3 block.
-__device__ __forceinline__ void store_token(const Params& P, const float (&y)[4], long long m, int n, int lane) {
-    const bool whole = n + 4 <= P.N;
-    if (P.out_dtype == EDB200_TYPE_F8_E4M3) {
-        float v[4] = {y[0], y[1], y[2], y[3]};
-        float a = row_peak(v, n, P.N);
+// What becomes of a token's finished features.
+enum { TO_F32, TO_STREAM, TO_F16, TO_BF16, TO_F8 };   // TO_STREAM: residual + gate * y
+
+// Four neighbouring features of token m in each lane of a warp: the 128 columns of one e4m3 block.  `whole`: all four exist.
+template <int TO>
+__device__ __forceinline__ void store_token(const Params& P, float (&y)[4], const float (&gate)[4], long long m, int n, bool whole,
+                                            int lane) {
+    if constexpr (TO == TO_F8) {
+        float a = row_peak(y, n, P.N);
 #pragma unroll
         for (int k = 16; k > 0; k >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, k));
         if (f8_has_infinity(a)) {   // uniform
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = f8_no_infinity(v[e]);
-            a = row_peak(v, n, P.N);
+            for (int e = 0; e < 4; ++e) y[e] = f8_no_infinity(y[e]);
+            a = row_peak(y, n, P.N);
 #pragma unroll
             for (int k = 16; k > 0; k >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, k));
         }
         float s, inv;
         f8_scale(a, s, inv);
-        const uint32_t w = f8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+        const uint32_t w = f8_pack4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
         uint8_t* o = static_cast<uint8_t*>(P.out) + m * P.ldo + n;
         if (whole) {
             *reinterpret_cast<uint32_t*>(o) = w;
@@ -277,42 +280,82 @@ __device__ __forceinline__ void store_token(const Params& P, const float (&y)[4]
             for (int e = 0; e < P.N - n; ++e) o[e] = static_cast<uint8_t>(w >> (8 * e));
         }
         if (lane == 0) P.out_scale[m * P.ld_os + (n >> 7)] = s;
-        return;
-    }
-    if (P.out_dtype == EDB200_TYPE_F32) {
+    } else if constexpr (TO == TO_F32 || TO == TO_STREAM) {
         float* o = static_cast<float*>(P.out) + m * P.ldo + n;
-        const float* q = P.residual + m * P.ld_res + n;   // read with a gate only
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (P.gate != nullptr && n + e < P.N) ? fmaf(__ldg(P.gate + n + e), y[e], q[e]) : y[e];
         if (whole) {
-            *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+            if (TO == TO_STREAM) {
+                const float4 q = *reinterpret_cast<const float4*>(P.residual + m * P.ld_res + n);
+                y[0] = fmaf(gate[0], y[0], q.x), y[1] = fmaf(gate[1], y[1], q.y);
+                y[2] = fmaf(gate[2], y[2], q.z), y[3] = fmaf(gate[3], y[3], q.w);
+            }
+            *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
         } else {
+            const float* q = P.residual + m * P.ld_res + n;   // read for TO_STREAM only
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (n + e < P.N) o[e] = v[e];
+            for (int e = 0; e < 3; ++e) {
+                if (n + e < P.N) o[e] = TO == TO_STREAM ? fmaf(gate[e], y[e], q[e]) : y[e];
             }
         }
-        return;
-    }
-    uint16_t h[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        h[e] = P.out_dtype == EDB200_TYPE_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(y[e])) : __half_as_ushort(__float2half_rn(y[e]));
-    }
-    uint16_t* o = static_cast<uint16_t*>(P.out) + m * P.ldo + n;
-    if (whole) {
-        *reinterpret_cast<uint2*>(o) = make_uint2(h[0] | (uint32_t(h[1]) << 16), h[2] | (uint32_t(h[3]) << 16));
     } else {
+        uint16_t h[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if (n + e < P.N) o[e] = h[e];
+            h[e] = TO == TO_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(y[e])) : __half_as_ushort(__float2half_rn(y[e]));
+        }
+        uint16_t* o = static_cast<uint16_t*>(P.out) + m * P.ldo + n;
+        if (whole) {
+            *reinterpret_cast<uint2*>(o) = make_uint2(h[0] | (uint32_t(h[1]) << 16), h[2] | (uint32_t(h[3]) << 16));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e) {
+                if (n + e < P.N) o[e] = h[e];
+            }
         }
     }
 }
 
+// A warp's share of a finished tile: tokens first, first + step, ..., four features a lane.  PARTS: CTAs whose sums are added
+// (at most), all of them asked for before the first is added.
+template <int TO, int PARTS>
+__device__ __forceinline__ void finish_rows(const Params& P, const float* sums, int pitch, int tokens, int m0, int n0, int first, int step,
+                                            int parts, int lane) {
+    const int n = n0 + 4 * lane;
+    const bool whole = n + 4 <= P.N;
+    float bias[4], gate[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        bias[e] = (P.bias != nullptr && n + e < P.N) ? __ldg(P.bias + n + e) : 0.0f;
+        gate[e] = (TO == TO_STREAM && n + e < P.N) ? __ldg(P.gate + n + e) : 0.0f;
+    }
+    const int end = P.M - m0 < tokens ? P.M - m0 : tokens;
+    for (int t = first; t < end; t += step) {
+        float4 v;
+        if constexpr (PARTS == 1) {
+            v = *reinterpret_cast<const float4*>(sums + t * pitch + 4 * lane);
+        } else {
+            float4 q[PARTS];
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                if (p < parts) q[p] = cluster_load4(sums + t * pitch + 4 * lane, p);
+            }
+            v = q[0];
+#pragma unroll
+            for (int p = 1; p < PARTS; ++p) {
+                if (p < parts) v.x += q[p].x, v.y += q[p].y, v.z += q[p].z, v.w += q[p].w;
+            }
+        }
+        float y[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
+        if (P.act != EDB200_ACT_NONE) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = act_one(y[e], P.act);
+        }
+        store_token<TO>(P, y, gate, m0 + t, n, whole, lane);
+    }
+}
+
 // The end of a tile shared by `parts` CTAs of a cluster: sums[token][128 features] lie in each one's shared memory; every
-// CTA finishes each parts-th token, a warp per token and four features a lane.
+// CTA finishes each parts-th token.  One loop for each output, chosen outside it: with the choice inside, a token cost 575
+// clocks.
 __device__ __forceinline__ void finish_tokens(const Params& P, const float* sums, int pitch, int tokens, int m0, int n0, int part,
                                               int parts, int warp, int warps, int lane, bool bad) {
     if (parts > 1) {
@@ -320,64 +363,53 @@ __device__ __forceinline__ void finish_tokens(const Params& P, const float* sums
     } else {
         __syncthreads();
     }
-    const int n = n0 + 4 * lane;
-    float bias[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) bias[e] = (P.bias != nullptr && n + e < P.N) ? __ldg(P.bias + n + e) : 0.0f;
-    // two tokens at a time, and every part's sums asked for before the first is added: the reads' latency is the time here
-    const int stride = parts * warps;
-    for (int t0 = part + parts * warp; t0 < tokens && m0 + t0 < P.M; t0 += 2 * stride) {
-        float4 q[2][8];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int t = t0 + i * stride < tokens ? t0 + i * stride : t0;
-            if (parts == 1) {
-                q[i][0] = *reinterpret_cast<const float4*>(sums + t * pitch + 4 * lane);
-            } else {
-#pragma unroll
-                for (int p = 0; p < 8; ++p) {
-                    if (p < parts) q[i][p] = cluster_load4(sums + t * pitch + 4 * lane, p);
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int t = t0 + i * stride;
-            float4 v = q[i][0];
-#pragma unroll
-            for (int p = 1; p < 8; ++p) {
-                if (p < parts) v.x += q[i][p].x, v.y += q[i][p].y, v.z += q[i][p].z, v.w += q[i][p].w;
-            }
-            float y[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
-            if (P.act != EDB200_ACT_NONE) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = act_one(y[e], P.act);
-            }
-            if (t < tokens && m0 + t < P.M && !bad) store_token(P, y, m0 + t, n, lane);   // uniform over the warp
-        }
+    const int first = bad ? tokens : part + parts * warp, step = parts * warps;   // after a wait that gave up: nothing
+    const int to = P.out_dtype == EDB200_TYPE_F32    ? (P.gate != nullptr ? TO_STREAM : TO_F32)
+                   : P.out_dtype == EDB200_TYPE_F16  ? TO_F16
+                   : P.out_dtype == EDB200_TYPE_BF16 ? TO_BF16
+                                                     : TO_F8;
+#define EDB_FINISH(TO)                                                                                \
+    if (parts == 1) {                                                                                 \
+        finish_rows<TO, 1>(P, sums, pitch, tokens, m0, n0, first, step, parts, lane);                 \
+    } else {                                                                                          \
+        finish_rows<TO, 8>(P, sums, pitch, tokens, m0, n0, first, step, parts, lane);                 \
     }
+    switch (to) {
+        case TO_F32: EDB_FINISH(TO_F32) break;
+        case TO_STREAM: EDB_FINISH(TO_STREAM) break;
+        case TO_F16: EDB_FINISH(TO_F16) break;
+        case TO_BF16: EDB_FINISH(TO_BF16) break;
+        default: EDB_FINISH(TO_F8) break;
+    }
+#undef EDB_FINISH
     if (parts > 1) cluster_sync_all();   // no CTA leaves while another reads its sums
 }
 
 // One group of scales: xs of 128 rows from m0 on, this lane's block `at`, as [row][8 of SCALE_PITCH], then ws of `halves` weight blocks.
-// Four rows of eight blocks a load; rows past the end follow the last one.
+// Four rows of eight blocks a load, AHEAD loads under way; rows past the end follow the last one.  A warp brings ROWS rows.
+template <int FIRST, int ROWS, int AHEAD>
 __device__ __forceinline__ void bring_scales(const Params& P, float* dst, int m0, int at, int n_block, int halves, int lane) {
     const int nb_last = (P.N - 1) >> 7;
-    if (lane < 8 * halves) {
+    if (FIRST == 0 && lane < 8 * halves) {
         const int nb = n_block + (lane >> 3);
         dst[128 * SCALE_PITCH + lane] = __ldg(P.ws + static_cast<long long>(nb < nb_last ? nb : nb_last) * P.ld_ws + at);
     }
-#pragma unroll 8
-    for (int i = 0; i < 32; ++i) {
-        const int r = 4 * i + (lane >> 3);
-        const int m = m0 + r < P.M ? m0 + r : P.M - 1;
-        dst[r * SCALE_PITCH + (lane & 7)] = __ldg(P.xs + m * P.ld_xs + at);
+    for (int j = FIRST / 4; j < (FIRST + ROWS) / 4; j += AHEAD) {
+        float x[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int r = 4 * (j + i) + (lane >> 3);
+            const int m = m0 + r < P.M ? m0 + r : P.M - 1;
+            x[i] = __ldg(P.xs + m * P.ld_xs + at);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) dst[(4 * (j + i) + (lane >> 3)) * SCALE_PITCH + (lane & 7)] = x[i];
     }
 }
 
 // ------------------------------------------------------------------ one CTA per 128 tokens x 128 features
 // For products whose 256 x 256 tiles are too few for the CTA pairs below.  Tokens in the lanes, features in the columns of
-// four accumulators; eight promotion warps of 32 tokens x 64 features, warp 2 bringing the scales as in the pairs.  Where
+// four accumulators; eight promotion warps of 32 tokens x 64 features, warps 2 and 3 bringing the scales as in the pairs.  Where
 // the tiles leave SMs idle a cluster of up to eight CTAs shares one, each a run of its k blocks; sums meet in shared memory
 // and are added in the order of the parts.
 namespace tile {
@@ -385,7 +417,7 @@ constexpr int STAGES = 5, BUFS = 4;
 constexpr int A_BYTES = 128 * BK, STAGE_BYTES = 2 * A_BYTES;
 constexpr int WARPS = 8;                                        // promotion warps
 constexpr int CPT = 64;                                         // columns of a promotion thread
-constexpr int THREADS = 32 * (WARPS + 4);                       // warp 0 TMA, 1 MMA, 2 scales, 4-11 promotion; all store
+constexpr int THREADS = 32 * (WARPS + 4);                       // warp 0 TMA, 1 MMA, 2 and 3 scales, 4-11 promotion; all store
 constexpr int SUM_PITCH = 132;                                  // words between rows of the sums (no conflicts)
 constexpr int SCALE_WORDS = 128 * SCALE_PITCH + 8;              // a group of eight blocks: [row][8], ws [8]
 constexpr int OFF_SCALE = STAGES * STAGE_BYTES;
@@ -426,7 +458,7 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             mbar_init(&acc_empty[i], WARPS);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sc_full[i], 1);
+            mbar_init(&sc_full[i], 2);
             mbar_init(&sc_empty[i], WARPS);
         }
         *abort_flag = 0;
@@ -486,12 +518,16 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 ph ^= 1u;
             }
         }
-    } else if (warp == 2) {
+    } else if (warp == 2 || warp == 3) {   // half of the rows' scales each
         for (int b = 0; b < blocks; b += 8) {
             const int g = b >> 3;
             if (!__all_sync(0xffffffffu, mbar_wait(&sc_empty[g & 1], ((g >> 1) & 1) ^ 1u, abort_flag, P.err))) break;
             const int at = b_first + (b + (lane & 7) < blocks ? b + (lane & 7) : blocks - 1);
-            bring_scales(P, scales + (g & 1) * SCALE_WORDS, m0, at, n_tile, 1, lane);
+            if (warp == 2) {
+                bring_scales<0, 64, 16>(P, scales + (g & 1) * SCALE_WORDS, m0, at, n_tile, 1, lane);
+            } else {
+                bring_scales<64, 64, 16>(P, scales + (g & 1) * SCALE_WORDS, m0, at, n_tile, 1, lane);
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sc_full[g & 1]);
         }
@@ -544,6 +580,17 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     if (warp == 1) {
         tc_fence_after_sync();
         tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// The residual rows of a CTA's 128 x 256 outputs into L2 while the products run (128 bytes a prefetch): the epilogue's loads
+// then wait for L2, not for memory.
+__device__ __forceinline__ void prefetch_residual(const Params& P, int m0, int n0, int lane) {
+    const int n = n0 + 32 * (lane & 7);
+    if (n >= P.N) return;
+    const int rows = P.M - m0 < 128 ? P.M - m0 : 128;
+    for (int r = lane >> 3; r < rows; r += 4) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(P.residual + static_cast<long long>(m0 + r) * P.ld_res + n));
     }
 }
 
@@ -796,9 +843,10 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     ok = __all_sync(0xffffffffu, mbar_wait(&sc_empty[sg & 1u], ((sg >> 1) & 1u) ^ 1u, abort_flag, P.err));
                     if (!ok) break;
                     const int at = b + (lane & 7) < P.kblocks ? b + (lane & 7) : P.kblocks - 1;
-                    bring_scales(P, dst0 + (sg & 1u) * SCALE_WORDS, m0, at, 2 * n_tile, 2, lane);
+                    bring_scales<0, 128, 16>(P, dst0 + (sg & 1u) * SCALE_WORDS, m0, at, 2 * n_tile, 2, lane);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sc_full[sg & 1u]);
+                    if (b == 0 && P.gate != nullptr) prefetch_residual(P, m0, n_tile * 256, lane);
                 }
             }
         } else if (warp == 1) {
@@ -1161,6 +1209,9 @@ extern "C" edb200_status_t edb200_mul_mat_fp8(const edb200_fp8_weight_t* w, cons
     if (ep->gate != nullptr && (dt != EDB200_TYPE_F32 || ep->residual == nullptr || (m > 1 && (ep->ld_res < w->n || ep->ld_res % 4)) ||
                                 (at(ep->residual) & 15u))) {
         return fail(EDB200_ERR_INVALID, "mul_mat_fp8: gated residual needs f32 out and residual rows of n values, 16-byte aligned");
+    }
+    if (ep->gate != nullptr && ep->out == ep->residual && m > 1 && ep->ldo != ep->ld_res) {
+        return fail(EDB200_ERR_INVALID, "mul_mat_fp8: out in the residual's place needs the same stride");
     }
     if (f8 != (out_scale != nullptr) || (f8 && ((m > 1 && ld_out_scale < nb) || (at(out_scale) & 3u)))) {
         return fail(EDB200_ERR_INVALID, "mul_mat_fp8: e4m3 out, and only it, needs out_scale with ceil(n / 128) columns");

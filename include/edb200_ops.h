@@ -359,7 +359,7 @@ EDB200_API edb200_status_t edb200_cast(const void* x, int in_dtype, void* y, int
  *   scale = a / 448,   q = e4m3(x * (448 / a)),   both divisions and the product rounded to f32, ties to even.
  * A value that is not finite becomes NaN and takes no part in a: an infinity is not turned into a number.
  * x [rows, ldx] f32 / f16 / bf16; q [rows, ldq] bytes; scale [ceil(rows / block_rows), ld_scale], of which
- * ceil(k / 128) columns are written.  Any rows >= 0, k >= 1, strides and element-aligned addresses; rows that
+ * ceil(k / 128) columns are written; q and x do not overlap.  Any rows >= 0, k >= 1, strides and element-aligned addresses; rows that
  * start on 16-byte boundaries take wide loads.  Columns of q beyond k are left as they were. */
 EDB200_API edb200_status_t edb200_quantize_fp8(const void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t k,
                                                int block_rows, void* q, int64_t ldq, float* scale, int64_t ld_scale,
@@ -384,7 +384,7 @@ typedef struct {
  * EDB200_TYPE_F8_E4M3: each row's activated columns are then quantised as edb200_quantize_fp8 does with
  * block_rows 1, bytes to ep->out and scales to out_scale [m, ld_out_scale], ready to be the next product's x;
  * split_n, split_k and pack are not available (EDB200_ERR_UNSUPPORTED).  Any m >= 0, n >= 1, k >= 1.
- * out_scale is NULL for the other output types. */
+ * out may be the residual (same stride) and overlaps nothing else; out_scale is NULL for the other output types. */
 EDB200_API edb200_status_t edb200_mul_mat_fp8(const edb200_fp8_weight_t* w, const void* x, const float* x_scale, int64_t m,
                                               int64_t ldx, int64_t ld_xs, const edb200_epilogue_t* ep, float* out_scale,
                                               int64_t ld_out_scale, void* stream);
@@ -401,7 +401,7 @@ EDB200_API edb200_status_t edb200_mul_mat_fp8(const edb200_fp8_weight_t* w, cons
  *   or single tokens with 1; rows_per_mod 0: one row for all.  NULL: 1, 0, 0.
  *   z_dtype EDB200_TYPE_F8_E4M3: z is quantised as edb200_quantize_fp8 does with block_rows 1, scales to
  *   z_scale [rows, ld_z_scale].
- * y may alias residual or x where type and stride agree.  h up to 16384, any strides; with h a multiple of four and
+ * y may be residual or x where type and stride agree; z overlaps none of them.  h up to 16384, any strides; with h a multiple of four and
  * every row of every buffer aligned to four of its elements, wide accesses.  Generalises edb200_layernorm_modulate and
  * edb200_fused_residual_gate, which keep the reference's order of operations bit for bit; this one does not. */
 enum { EDB200_NORM_NONE = 0, EDB200_NORM_LAYER = 1, EDB200_NORM_RMS = 2 };

@@ -158,6 +158,7 @@ def test_mul_mat_refusals(edb):
     refused(edb, call(ep=epilogue(edb, gate=4096)), "gated")
     refused(edb, call(ep=epilogue(edb, gate=4096, out_dtype=edb.TYPE_F32)), "gated")
     refused(edb, call(ep=epilogue(edb, gate=4096, out_dtype=edb.TYPE_F32, residual=4096, ld_res=258)), "gated")
+    refused(edb, call(ep=epilogue(edb, gate=4096, out_dtype=edb.TYPE_F32, residual=4096, ld_res=260)), "residual's place")
     refused(edb, call(ep=epilogue(edb, out_dtype=edb.TYPE_F8_E4M3)), "out_scale")
     refused(edb, call(os=4096, ld_os=2), "out_scale")
     refused(edb, call(ep=epilogue(edb, out_dtype=edb.TYPE_F8_E4M3), os=4096, ld_os=1), "out_scale")
@@ -424,6 +425,67 @@ def test_mul_mat_quantised_output_of_rows_not_finite(edb, cuda, m):
     plain[:, 3] = 0.0
     top = blocked(plain, 1, torch.float64).abs().amax((1, 3))
     assert bool(((ys.double() * 448 - top).abs() <= top * 2.0 ** -12).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(2, 12800, 256), (40, 9000, 130), (130, 20480, 200), (200, 1400, 300), (600, 2304, 5300),
+                                   (2600, 500, 2100), (19000, 130, 260)])
+def test_mul_mat_long_sums_and_many_tiles(edb, cuda, m, k, n):
+    """k split over clusters, groups of eight blocks that end early, tiles walked by resident CTA pairs in chunks."""
+    run_linear(edb, m, k, n, torch.float32, seed=k)
+    run_linear(edb, m, k, n, "f8", act="silu", seed=k + 1)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(edb, cuda):
+    """Rows so far apart that a row's offset passes 2^32 bytes and 2^31 elements."""
+    far, rows, k = (1 << 30) + 64, 3, 256
+    big = torch.empty(2 * far + 4096, device="cuda", dtype=torch.float16)
+    x = big.as_strided((rows, k), (far, 1))
+    x.copy_(randn(rows, k, seed=3))
+    q, s = torch.empty(rows, k, device="cuda", dtype=F8), torch.empty(rows, 2, device="cuda")
+    edb.quantize_fp8(x, q, s)
+    want_q, want_s = quantize_plain(x.contiguous(), 1)
+    assert torch.equal(bits(q.cpu()), bits(want_q)) and torch.equal(s.cpu(), want_s)
+    wq, ws = fp8_operand(n := 384, k, 128, 7, 0, 0.05)
+    want, err = linear64(q, s, wq, ws, None, "none")
+    y = big.as_strided((rows, n), (far, 1), 512)
+    edb.mul_mat_fp8(edb.Fp8Weight(wq, ws), q, s, edb.make_epilogue(y))
+    assert bool(((y.double() - want).abs() <= err + (want.abs() + err) * UNIT[torch.float16] + TINY[torch.float16]).all())
+    z = big.as_strided((rows, k), (far, 1), 1024)
+    edb.block_norm(x, z, None, residual_scale=2.0)
+    assert torch.equal(z, x * 2)
+    t = big.as_strided((rows, 2, 128), (far, 128, 1), 2048)
+    edb.Rope([128]).apply(None, x.unflatten(1, (2, 128)), t)
+    assert torch.equal(t[0].flatten(), x[0])
+    small = torch.empty(rows, 2, 128, device="cuda", dtype=torch.float16)
+    edb.Rope([128]).apply(None, x.contiguous().unflatten(1, (2, 128)), small)
+    assert torch.equal(t, small)
+
+
+@pytest.mark.gpu
+def test_two_streams_and_two_recordings_at_once(edb, cuda):
+    """No call keeps anything outside its arguments: the same products from two streams, eager and recorded, side by side."""
+    m, k, n = 300, 1280, 1100
+    xq, xs = fp8_operand(m, k, 1, 1)
+    wq, ws = fp8_operand(n, k, 128, 2, 0, 0.05)
+    w = edb.Fp8Weight(wq, ws)
+    outs = [torch.empty(m, 1104, device="cuda")[:, :n] for _ in range(5)]
+    edb.mul_mat_fp8(w, xq, xs, edb.make_epilogue(outs[4]))
+    torch.cuda.synchronize()
+    streams, graphs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for i, st in enumerate(streams):
+        with torch.cuda.stream(st):
+            graphs.append(edb.Graph(lambda i=i: edb.mul_mat_fp8(w, xq, xs, edb.make_epilogue(outs[i]))))
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                graphs[i].launch()
+                edb.mul_mat_fp8(w, xq, xs, edb.make_epilogue(outs[2 + i]))
+    torch.cuda.synchronize()
+    edb.poll_status()
+    for o in outs[:4]:
+        assert torch.equal(o, outs[4])
 
 
 # ----------------------------------------------------------------------------------------------------- block_norm
