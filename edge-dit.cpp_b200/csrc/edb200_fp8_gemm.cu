@@ -408,7 +408,7 @@ __device__ __forceinline__ void bring_scales(const Params& P, float* dst, int m0
 }
 
 // ------------------------------------------------------------------ one CTA per 128 tokens x 128 features
-// For products whose 256 x 256 tiles are too few for the CTA pairs below.  Tokens in the lanes, features in the columns of
+// For products whose 256 x 256 tiles are too few for the CTA pairs below (256 x 5120 x 5120 20 us; pairs 28).  Tokens in the lanes, features in the columns of
 // four accumulators; eight promotion warps of 32 tokens x 64 features, warps 2 and 3 bringing the scales as in the pairs.  Where
 // the tiles leave SMs idle a cluster of up to eight CTAs shares one, each a run of its k blocks; sums meet in shared memory
 // and are added in the order of the parts.
@@ -597,17 +597,20 @@ __device__ __forceinline__ void prefetch_residual(const Params& P, int m0, int n
 // ------------------------------------------------------ CTA pairs: 256 tokens x 256 features, one pair per two SMs
 // The leader's MMAs span both CTAs (cta_group::2): each stages its own 128 tokens and half of the 256 features, so an
 // SM takes in 32 KB for 512 clocks of tensor work.  The two 128-feature halves of a block are MMAs and accumulators of
-// their own: all 512 tensor-memory columns hold [half][2 alternating][128], and a half's accumulator is due again only
-// three MMA groups (768 clocks) after it was finished - with one 256-column pair of accumulators the tensor pipe waited
-// for the reading of the last one half of the time.  Each of eight promotion warps owns 32 tokens x one half, which is
-// one weight block and, for e4m3 output, one quantisation block.
+// their own: all 512 tensor-memory columns hold [half][2 alternating][128].  Each of eight promotion warps owns 32 tokens x
+// one half, which is one weight block and, for e4m3 output, one quantisation block; it asks for 64 columns at a time and
+// gives the accumulator back before it adds the second 64.  Sixteen warps of half the columns were slower (1.63 against 1.9
+// PFLOP/s), and so was one 256-column accumulator for both halves.
 // Each half has an issuer of its own (warps 1 and 2 of the leader): waiting, issuing and committing are a chain of about
 // 250 clocks a group for one thread, twice that per block for a common one.
 // Warp 3 brings the scales, eight blocks of the CTA's 128 rows at a time, two groups in shared memory.  The promotion
-// warps touch no global memory while they add: with one load in flight each of their tensor-memory reads waited for
-// it (1060 clocks a block instead of 650).
+// warps touch no global memory while they add: tcgen05.wait::ld waited for their loads, too, and a block took 1060 clocks
+// instead of 780.
 // Signals across the pair: the peer's warp 1 passes its full barriers on to the leader's (two arrivals there: own copies,
 // peer's); acc_empty counts the promotion warps of both CTAs; the commits arrive in both.
+// Measured: 32760 x 5120 x 13824 into f16 2.4 ms (1.9 PFLOP/s), 32760 x 13824 x 5120 into the stream 2.4 ms; loads and
+// MMAs alone 1.46 ms, MMAs alone 1.17.  Bound by the loop MMA - commit - reading - signal - MMA: two blocks an accumulator
+// pair take about 1900 clocks, of which 512 are MMAs of the half, 550 the reading, and the signals between the SMs the rest.
 namespace pair {
 constexpr int STAGES = 5;
 constexpr int A_BYTES = 128 * BK, B_HALF = 64 * BK, STAGE_BYTES = A_BYTES + 2 * B_HALF;
@@ -877,7 +880,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 }
 
 // ----------------------------------------------------------- few rows: 128 features x NT tokens, k split over a cluster
-// Bound: HBM, the weights read once.  The roles are turned round: features lie in the 128 lanes of tensor memory, tokens in
+// Bound: HBM, the weights read once (2 x 5120 x 30720 29 us, 5.4 TB/s, 0.83 of the copy rate).  The roles are turned round: features lie in the 128 lanes of tensor memory, tokens in
 // its columns, so that a tile wastes nothing on tokens that are not there; a column's scale is then one number per token
 // and block, laid out by warp 2 for eight blocks at a time.  Two CTAs share an SM and keep 160 KB of weights under way
 // there.  Where the tiles alone leave SMs idle, a cluster of up to eight CTAs takes a tile, each a run of its k blocks; the
