@@ -7,13 +7,14 @@
 //
 // Bound: HBM.  A row's x and residual are read once, live in registers through both norms, and y and z are written
 // once; the statistics are f32 sums over registers, the variance taken around the mean (two sums, no cancellation).
-// A row belongs to one warp (h <= 1024, eight rows a CTA, sums by shuffles alone) or to one CTA of just as many warps as it
+// A row belongs to one warp (h <= 512, eight rows a CTA, sums by shuffles alone) or to one CTA of just as many warps as it
 // needs.  A warp owns CH blocks of 128 columns, a lane four columns of each: every access of a warp is one run of memory
 // (eight columns a lane took twice the f32 wavefronts), the places differ by constants, and a quantisation block's
-// maximum is one reduction over the warp.  Two blocks a warp: with four, the vectors' loads in flight took the registers
-// of half the rows (423 against 388 us at the first size below).
-// Measured (f32 stream): 32760 x 5120 bf16 normed on both sides into e4m3 388 us (4.75 TB/s, 0.72 of the copy rate),
-// LayerNorm into f16 345 us (5.83 TB/s, 0.89), 154 x 1536 3.5 us.
+// maximum is one reduction over the warp.  Four blocks a warp and 64 registers a thread keep three rows of 5120 under way on
+// an SM (310 us at the first size below; two blocks a warp, one row: 388); where there are fewer rows than that, two blocks
+// a warp finish a row sooner (1 x 5120: 3.7 against 4.0 us).
+// Measured (f32 stream): 32760 x 5120 bf16 normed on both sides into e4m3 310 us (6.0 TB/s, 0.91 of the copy rate),
+// LayerNorm into f16 298 us (6.8 TB/s), 154 x 1536 3.5 us.
 #include "edb200_internal.h"
 #include "edb200_fp8.cuh"
 
@@ -304,21 +305,20 @@ template <typename TX, typename TS>
 static void launch_vec(const Params& P, bool vec, cudaStream_t s) {
     const int64_t rows = P.p.rows;
     const int blocks = static_cast<int>((P.p.h + 127) / 128);
-    if (blocks <= 8) {
+    if (blocks <= 4) {
         const unsigned grid = static_cast<unsigned>((rows + 7) / 8);
         if (blocks <= 2) {
             launch_access<TX, TS, 2, true>(P, vec, grid, 256, s);
-        } else if (blocks <= 4) {
-            launch_access<TX, TS, 4, true>(P, vec, grid, 256, s);
         } else {
-            launch_access<TX, TS, 8, true>(P, vec, grid, 256, s);
+            launch_access<TX, TS, 4, true>(P, vec, grid, 256, s);
         }
-    } else if (blocks <= 64) {
+    } else if (blocks <= 64 && rows <= 2 * sm_count()) {
         launch_access<TX, TS, 2, false>(P, vec, static_cast<unsigned>(rows), 32u * ((blocks + 1) / 2), s);
     } else {
         launch_access<TX, TS, 4, false>(P, vec, static_cast<unsigned>(rows), 32u * ((blocks + 3) / 4), s);
     }
 }
+
 template <typename TS>
 static void launch_x(const Params& P, bool vec, cudaStream_t s) {
     if (P.p.x == nullptr || P.p.x_dtype == EDB200_TYPE_F32) {
