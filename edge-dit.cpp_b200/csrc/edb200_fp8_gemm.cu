@@ -499,8 +499,8 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         uint32_t s = 0, ph = 0;
         for (int b = 0; b < blocks; ++b) {
             const uint32_t buf = b % BUFS, aph = (b / BUFS) & 1u;
-            if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag, P.err)) break;
             if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
+            if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag, P.err)) break;
             tc_fence_after_sync();
             if (elect_one()) {
                 const uint32_t a_addr = smem_u32(smem + s * STAGE_BYTES), b_addr = a_addr + A_BYTES;
@@ -815,15 +815,17 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             uint32_t s = 0, ph = 0;
             for (int g = 0; g < blocks; ++g) {   // k blocks of all this pair's tiles
                 const uint32_t buf = g & 1u, aph = (g >> 1) & 1u;
-                if (!mbar_wait(&acc_empty[2 * half + buf], aph ^ 1u, abort_flag, P.err)) break;
+                // the stage first: it is there long before the accumulator, whose signal should find nothing left to wait for
                 if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
+                const uint32_t d = tmem_base + half * 256 + buf * 128;
+                const uint32_t off = s * (STAGE_BYTES >> 4);   // descriptors count 16-byte units
+                const uint64_t a_desc = a_desc0 + off, b_desc = b_desc0 + off;
+                if (!mbar_wait(&acc_empty[2 * half + buf], aph ^ 1u, abort_flag, P.err)) break;
                 tc_fence_after_sync();
                 if (elect_one()) {
-                    const uint32_t d = tmem_base + half * 256 + buf * 128;
-                    const uint32_t off = s * (STAGE_BYTES >> 4);   // descriptors count 16-byte units
 #pragma unroll
                     for (int j = 0; j < BK / 32; ++j) {
-                        mma_f8_ss_pair(d, a_desc0 + off + 2 * j, b_desc0 + off + 2 * j, idesc, j > 0 ? 1u : 0u);
+                        mma_f8_ss_pair(d, a_desc + 2 * j, b_desc + 2 * j, idesc, j > 0 ? 1u : 0u);
                     }
                     mma_commit_pair(&acc_full[2 * half + buf]);
                     mma_commit_pair(&empty[s]);
@@ -977,8 +979,8 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         uint32_t s = 0, ph = 0;
         for (int b = 0; b < blocks; ++b) {
             const uint32_t buf = b % L::BUFS, aph = (b / L::BUFS) & 1u;
-            if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag, P.err)) break;
             if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
+            if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag, P.err)) break;
             tc_fence_after_sync();
             if (elect_one()) {
                 const uint32_t a_addr = smem_u32(smem + s * L::STAGE_BYTES), b_addr = a_addr + W_BYTES;
