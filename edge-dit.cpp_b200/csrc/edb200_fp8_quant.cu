@@ -68,28 +68,40 @@ __device__ __forceinline__ float group_max(float a) {
     return a;
 }
 
-// 1 x 128: a group of eight lanes per block; I is the index type that holds rows * blocks.
-template <typename T, bool VEC, typename I>
+// 1 x 128: a group of eight lanes per block.  SMALL: the block's row by the product with 2^32 / kb rounded up, exact while
+// blocks times kb stay below 2^32; else by division in 64 bits.
+template <typename T, bool VEC, bool SMALL>
 __global__ void __launch_bounds__(THREADS)
-quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int k, int kb, uint8_t* __restrict__ q, int64_t ldq,
-                     float* __restrict__ scale, int64_t ld_scale) {
+quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int k, int kb, uint32_t inv_kb, uint8_t* __restrict__ q,
+                     int64_t ldq, float* __restrict__ scale, int64_t ld_scale) {
     const int l = threadIdx.x & 7;
-    const I g = static_cast<I>(blockIdx.x) * (THREADS / 8) + (threadIdx.x >> 3);
-    const I row = g / static_cast<I>(kb);
-    const int b = static_cast<int>(g - row * static_cast<I>(kb));
-    const bool live = static_cast<int64_t>(row) < rows;
+    int64_t row;
+    int b;
+    if (SMALL) {
+        const uint32_t g = blockIdx.x * (THREADS / 8) + (threadIdx.x >> 3);
+        const uint32_t r = kb == 1 ? g : __umulhi(g, inv_kb);
+        row = r;
+        b = static_cast<int>(g - r * static_cast<uint32_t>(kb));
+    } else {
+        const int64_t g = static_cast<int64_t>(blockIdx.x) * (THREADS / 8) + (threadIdx.x >> 3);
+        row = g / kb;
+        b = static_cast<int>(g - row * kb);
+    }
+    const bool live = row < rows;
     float v[16];
-    load16<T, VEC>(x + static_cast<int64_t>(row) * ldx, b * 128, l, k, live, v);
+    load16<T, VEC>(x + row * ldx, b * 128, l, k, live, v);
     float a = group_max(peak16(v));
-    uint8_t* qr = q + static_cast<int64_t>(row) * ldq;
     if (__any_sync(0xffffffffu, f8_has_infinity(a))) {   // some block of the warp holds an infinity
         no_infinities16(v);
         a = group_max(peak16(v));
     }
-    float s, inv;
-    f8_scale(a, s, inv);
-    if (live) store16<VEC>(qr, b * 128, l, k, v, inv);
-    if (live && l == 0) scale[static_cast<int64_t>(row) * ld_scale + b] = s;
+    // f8_scale()'s two divisions as one: the group's first lane makes the scale, the others its inverse
+    a = fmaxf(a, kF8Floor);
+    const float quotient = __fdiv_rn(l == 0 ? a : kF8Max, l == 0 ? kF8Max : a);
+    const float inv = __shfl_sync(0xffffffffu, quotient, (threadIdx.x & 24) | 1);
+    if (!live) return;
+    store16<VEC>(q + row * ldq, b * 128, l, k, v, inv);
+    if (l == 0) scale[row * ld_scale + b] = quotient;
 }
 
 template <int N>
@@ -154,15 +166,15 @@ static edb200_status_t launch(const T* x, int64_t ldx, int64_t rows, int64_t k, 
         const int64_t ctas = (groups + THREADS / 8 - 1) / (THREADS / 8);
         if (ctas > 0x7fffffff) return fail(EDB200_ERR_UNSUPPORTED, "quantize_fp8: more than 2^36 blocks");
         const unsigned grid = static_cast<unsigned>(ctas);
-        // 32-bit block indices where they hold every block of the grid: one division less in 64 bits per thread
-        if (groups < 0x7fffff00ll) {
-            if (vec) {
-                quantize_rows_kernel<T, true, uint32_t><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, (int)kb, q, ldq, scale, ld_scale);
-            } else {
-                quantize_rows_kernel<T, false, uint32_t><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, (int)kb, q, ldq, scale, ld_scale);
-            }
+        const int kbi = static_cast<int>(kb);
+        const uint32_t inv_kb = static_cast<uint32_t>((0x100000000ull + kb - 1) / kb);
+        const bool small = static_cast<double>(ctas) * (THREADS / 8) * static_cast<double>(kb) < 4294967296.0;
+        if (!small) {
+            quantize_rows_kernel<T, false, false><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, kbi, inv_kb, q, ldq, scale, ld_scale);
+        } else if (vec) {
+            quantize_rows_kernel<T, true, true><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, kbi, inv_kb, q, ldq, scale, ld_scale);
         } else {
-            quantize_rows_kernel<T, false, uint64_t><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, (int)kb, q, ldq, scale, ld_scale);
+            quantize_rows_kernel<T, false, true><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, kbi, inv_kb, q, ldq, scale, ld_scale);
         }
     } else {
         const int64_t rb = (rows + 127) / 128;

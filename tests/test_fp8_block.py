@@ -263,6 +263,18 @@ def test_quantize(edb, cuda, dtype, rows, k, block_rows, pad, skew):
 
 
 @pytest.mark.gpu
+def test_quantize_rows_of_many_blocks(edb, cuda):
+    """So many blocks a row that a block's row is found by division in 64 bits: 11 x 20001 blocks."""
+    rows, k = 11, 20000 * 128 + 5
+    x = laid(randn(rows, k, seed=5), torch.float16)
+    q, s = blank(rows, k, F8), blank(rows, 20001, torch.float32, 1)
+    edb.quantize_fp8(x, q, s)
+    want_q, want_s = quantize_plain(x, 1)
+    assert torch.equal(bits(q.cpu()), bits(want_q)) and torch.equal(s.cpu(), want_s)
+    assert margins_untouched(q) and margins_untouched(s)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("block_rows", [1, 128])
 def test_quantize_extremes(edb, cuda, block_rows):
     """Zero blocks, tiny and huge magnitudes, values that are not finite: only those become NaN."""
