@@ -462,6 +462,8 @@ def quantize_fp8(x, q, scale, block_rows=1):
     """q (float8_e4m3fn, like x [rows, k]) and scale (float32 [ceil(rows / block_rows), ceil(k / 128)]) of x:
     edb200_quantize_fp8 on the current stream."""
     rows, k = x.shape
+    if block_rows != 1 and block_rows != 128:
+        raise ValueError("quantize_fp8: block_rows must be 1 or 128")
     if q.shape != x.shape or torch_dtype_id(q) != TYPE_F8_E4M3:
         raise ValueError("quantize_fp8: q must be float8_e4m3fn of x's shape")
     lds = _scale_rows(scale, -(-rows // block_rows), -(-k // 128), "quantize_fp8: scale")
@@ -509,7 +511,8 @@ def block_norm(residual, y=None, z=None, z_scale=None, x=None, gate=None, residu
     rows, h = shape
     stream_id = torch_dtype_id(residual)
     px = py = pz = pzs = pg = psc = psh = None
-    ldx = ldy = ldz = ldzs = ld_mod = x_id = z_id = 0
+    ldx = ldy = ldz = ldzs = x_id = z_id = 0
+    ld_mod = None
     if x is not None:
         if x.shape != shape:
             raise ValueError("block_norm: x must have residual's shape")
@@ -526,13 +529,13 @@ def block_norm(residual, y=None, z=None, z_scale=None, x=None, gate=None, residu
         pzs, ldzs = z_scale.data_ptr(), _scale_rows(z_scale, rows, -(-h // 128), "block_norm: z_scale")
     groups = -(-rows // rows_per_mod) if rows_per_mod else 1
     if gate is not None:
-        pg, ld_mod = _modulation(gate, groups, h, 0)
+        pg, ld_mod = _modulation(gate, groups, h, None)
     if scale is not None:
         psc, ld_mod = _modulation(scale, groups, h, ld_mod)
     if shift is not None:
         psh, ld_mod = _modulation(shift, groups, h, ld_mod)
     d = BlockNormDesc(rows, h, px, ldx, residual.data_ptr(), _rows_of(residual, "residual"), py, ldy, pz, ldz, pzs, ldzs,
-                      pg, psc, psh, ld_mod, rows_per_mod, _affine(post_weight, h), _affine(post_bias, h),
+                      pg, psc, psh, ld_mod or 0, rows_per_mod, _affine(post_weight, h), _affine(post_bias, h),
                       _affine(pre_weight, h), _affine(pre_bias, h), residual_scale, post_eps, pre_eps, x_id, stream_id,
                       z_id, post_norm, pre_norm)
     st = lib().edb200_block_norm(C.byref(d), _launch_stream((residual, x, y, z, z_scale, gate, scale, shift, post_weight,
@@ -542,7 +545,7 @@ def block_norm(residual, y=None, z=None, z_scale=None, x=None, gate=None, residu
 
 
 def _modulation(t, groups, h, ld):
-    """Address and row stride of `groups` float32 rows of h values, which share one stride."""
+    """Address and row stride of `groups` float32 rows of h values, which share one stride (ld: the stride so far)."""
     shape = t.shape
     if len(shape) == 1 and groups == 1 and shape[0] == h:
         at = h
@@ -552,7 +555,7 @@ def _modulation(t, groups, h, ld):
         raise ValueError(f"block_norm: gate, scale and shift must be float32 [{groups}, {h}]")
     if torch_dtype_id(t) != TYPE_F32 or (len(shape) == 1 and not t.is_contiguous()):
         raise ValueError(f"block_norm: gate, scale and shift must be float32 [{groups}, {h}]")
-    if groups > 1 and ld and at != ld:
+    if groups > 1 and ld is not None and at != ld:
         raise ValueError("block_norm: gate, scale and shift must share one row stride")
     return t.data_ptr(), at
 

@@ -359,7 +359,8 @@ EDB200_API edb200_status_t edb200_cast(const void* x, int in_dtype, void* y, int
  *   scale = a / 448,   q = e4m3(x * (448 / a)),   both divisions and the product rounded to f32, ties to even.
  * A value that is not finite becomes NaN and takes no part in a: an infinity is not turned into a number.
  * x [rows, ldx] f32 / f16 / bf16; q [rows, ldq] bytes; scale [ceil(rows / block_rows), ld_scale], of which
- * ceil(k / 128) columns are written; q and x do not overlap.  Any rows >= 0, k >= 1, strides and element-aligned addresses; rows that
+ * ceil(k / 128) columns are written; q and x do not overlap.  Any rows >= 0 (with
+ * block_rows 128 up to 65535 x 128), k >= 1, strides and element-aligned addresses; rows that
  * start on 16-byte boundaries take wide loads.  Columns of q beyond k are left as they were. */
 EDB200_API edb200_status_t edb200_quantize_fp8(const void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t k,
                                                int block_rows, void* q, int64_t ldq, float* scale, int64_t ld_scale,

@@ -241,6 +241,53 @@ def test_rope_refusals(edb):
     assert call(tokens=0, q=dict(in_=None)) == edb.OK
 
 
+@pytest.mark.gpu
+def test_binding_refusals(edb, cuda):
+    """What the binding sees before the library: shapes, types, strides, places."""
+    t = lambda *s, dt=torch.float32: torch.zeros(*s, device="cuda", dtype=dt)  # noqa: E731
+    x, q, s = t(4, 256), t(4, 256, dt=F8), t(4, 2)
+    for bad in (dict(x=x.cpu()), dict(q=t(4, 255, dt=F8)), dict(q=t(4, 256)), dict(scale=t(4, 3)), dict(scale=t(4, 2, dt=torch.float16)),
+                dict(x=t(256, 4).t()), dict(block_rows=64)):
+        with pytest.raises(ValueError):
+            edb.quantize_fp8(**{**dict(x=x, q=q, scale=s), **bad})
+    with pytest.raises(edb.EdbError):                        # one row for all of them: no stride
+        edb.quantize_fp8(t(1, 256).expand(4, 256), q, s)
+    with pytest.raises(ValueError):
+        edb.Fp8Weight(t(128, 256, dt=F8), t(2, 2))
+    w = edb.Fp8Weight(t(128, 256, dt=F8), t(1, 2))
+    ep = edb.make_epilogue(t(4, 128))
+    for bad in (dict(x=t(4, 240, dt=F8)), dict(x=x), dict(x_scale=t(4, 1)), dict(out_scale=t(4, 2)), dict(x_scale=s.cpu())):
+        with pytest.raises(ValueError):
+            edb.mul_mat_fp8(**{**dict(w=w, x=q, x_scale=s, ep=ep), **bad})
+    r, y = t(4, 256), t(4, 256)
+    for bad in (dict(y=t(4, 255)), dict(y=t(4, 256, dt=torch.float16)), dict(x=t(3, 256)), dict(z=t(4, 128)), dict(z_scale=t(4, 1)),
+                dict(gate=t(255)), dict(gate=t(256, dt=torch.float16)), dict(gate=t(1, 256), rows_per_mod=2), dict(post_weight=t(255)),
+                dict(gate=t(1, 256).expand(4, 256), scale=t(4, 256), rows_per_mod=1), dict(pre_bias=t(512)[::2]),
+                dict(scale=t(4, 256), shift=t(4, 260)[:, :256], rows_per_mod=1), dict(gate=t(256).cpu())):
+        with pytest.raises(ValueError):
+            edb.block_norm(**{**dict(residual=r, y=y), **bad})
+    with pytest.raises(edb.EdbError):
+        edb.block_norm(r, y, x=r, gate=t(1, 256).expand(4, 256), rows_per_mod=1)
+    rope, a = edb.Rope([64]), t(4, 2, 64)
+    pos = torch.zeros(4, 1, device="cuda", dtype=torch.int32)
+    for bad in (dict(q_out=t(4, 2, 63)), dict(q_out=t(4, 2, 64, dt=torch.float16)), dict(positions=pos.long()), dict(positions=pos[:3]),
+                dict(k=t(3, 2, 64), k_out=t(3, 2, 64)), dict(q=t(4, 64, 2).transpose(1, 2)), dict(positions=pos.cpu())):
+        with pytest.raises(ValueError):
+            rope.apply(**{**dict(positions=pos, q=a, q_out=a), **bad})
+
+
+@pytest.mark.gpu
+def test_nothing_to_do(edb, cuda):
+    """No rows, no tokens: nothing is read, written or launched."""
+    t = lambda *s, dt=torch.float32: torch.zeros(*s, device="cuda", dtype=dt)  # noqa: E731
+    n0 = edb.lib().edb200_launch_count()
+    edb.quantize_fp8(t(0, 256), t(0, 256, dt=F8), t(0, 2))
+    edb.mul_mat_fp8(edb.Fp8Weight(t(128, 256, dt=F8), t(1, 2)), t(0, 256, dt=F8), t(0, 2), edb.make_epilogue(t(0, 128)))
+    edb.block_norm(t(0, 256), t(0, 256))
+    edb.Rope([64]).apply(None, t(0, 2, 64), t(0, 2, 64))
+    assert edb.lib().edb200_launch_count() == n0
+
+
 # ------------------------------------------------------------------------------------------------------- quantize
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
