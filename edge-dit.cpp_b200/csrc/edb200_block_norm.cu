@@ -11,10 +11,10 @@
 // needs.  A warp owns CH blocks of 128 columns, a lane four columns of each: every access of a warp is one run of memory
 // (eight columns a lane took twice the f32 wavefronts), the places differ by constants, and a quantisation block's
 // maximum is one reduction over the warp.  Four blocks a warp and 64 registers a thread keep three rows of 5120 under way on
-// an SM (310 us at the first size below; two blocks a warp, one row: 388); where there are fewer rows than that, two blocks
+// an SM (308 us at the first size below; two blocks a warp, one row: 388); where there are fewer rows than that, two blocks
 // a warp finish a row sooner (1 x 5120: 3.7 against 4.0 us).
-// Measured (f32 stream): 32760 x 5120 bf16 normed on both sides into e4m3 310 us (6.0 TB/s, 0.91 of the copy rate),
-// LayerNorm into f16 298 us (6.8 TB/s), 154 x 1536 3.5 us.
+// Measured (f32 stream): 32760 x 5120 bf16 normed on both sides into e4m3 308 us (6.0 TB/s, 0.91 of the copy rate; 329
+// where the allocator placed the operands otherwise), LayerNorm into f16 299-309 us (6.5-6.7 TB/s), 154 x 1536 3.5 us.
 #include "edb200_internal.h"
 #include "edb200_fp8.cuh"
 
@@ -96,7 +96,8 @@ __device__ __forceinline__ void store_piece(T* row, int c, int h, const float2 (
 }
 
 // 1 / sqrt(a): the hardware's approximation and one Newton step, which takes its two roundings' error down to one.  An e4m3 z
-// shows them wherever a value lies next to a border.  (The correctly rounded functions cost 15 % of the kernel.)
+// shows them wherever a value lies next to a border.  (It costs nothing measurable; the correctly rounded functions
+// cost 15 % of the kernel.)
 __device__ __forceinline__ float inverse_root(float a) {
     const float r = rsqrtf(a);
     const float e = fmaf(-a * r, r, 1.0f);

@@ -6,7 +6,7 @@
 // Eight lanes own one row's 128 columns: lane l takes columns 64 j + 8 l .. + 7 (j = 0, 1), so a warp's load of
 // 16-bit values is four full 128-byte lines and the block maximum is three shuffles.  What else bounded it was the number of
 // instructions a value: with a test for infinities on each (now on a block's maximum) 16-bit rows ran at 4.1 TB/s.
-// Measured: 32760 x 5120 bf16 rows 86 us (5.8 TB/s, 0.89 of the copy rate), 13824 x 5120 f32 in 128 x 128 blocks 53 us
+// Measured: 32760 x 5120 bf16 rows 84 us (6.0 TB/s, 0.91 of the copy rate), 13824 x 5120 f32 in 128 x 128 blocks 53 us
 // (6.7 TB/s), the same from bf16 51 us (4.2 TB/s: a CTA loads, reduces and stores in turn, three to an SM).
 #include "edb200_internal.h"
 #include "edb200_fp8.cuh"
