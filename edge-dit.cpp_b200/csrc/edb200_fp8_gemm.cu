@@ -385,25 +385,39 @@ __device__ __forceinline__ void finish_tokens(const Params& P, const float* sums
     if (parts > 1) cluster_sync_all();   // no CTA leaves while another reads its sums
 }
 
-// One group of scales: xs of 128 rows from m0 on, this lane's block `at`, as [row][8 of SCALE_PITCH], then ws of `halves` weight blocks.
-// Four rows of eight blocks a load, AHEAD loads under way; rows past the end follow the last one.  A warp brings ROWS rows.
-template <int FIRST, int ROWS, int AHEAD>
-__device__ __forceinline__ void bring_scales(const Params& P, float* dst, int m0, int at, int n_block, int halves, int lane) {
+// Copies of four bytes from global to shared memory that hold no register while they are under way.  `in` false: nothing is
+// read, zero is written (src is any address).
+__device__ __forceinline__ void copy4(float* dst, const float* src, bool in = true) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+// Waits for this thread's; the warp's after a __syncwarp.
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Starts the copy of one group of scales: xs of 128 rows from m0 on, this lane's block `at`, as [row][8 of SCALE_PITCH], then ws of
+// `halves` weight blocks.  Four rows of eight blocks a copy; rows past the end follow the last one.  A warp brings ROWS
+// rows.  (By loads, as many under way as registers allow, a change elsewhere in the kernel that left the compiler one
+// register less put them one behind the other: 600 x 4096 x 1024 17 us instead of 12.)
+template <int FIRST, int ROWS>
+__device__ __forceinline__ void copy_scales(const Params& P, float* dst, int m0, int at, int n_block, int halves, int lane) {
     const int nb_last = (P.N - 1) >> 7;
     if (FIRST == 0 && lane < 8 * halves) {
         const int nb = n_block + (lane >> 3);
-        dst[128 * SCALE_PITCH + lane] = __ldg(P.ws + static_cast<long long>(nb < nb_last ? nb : nb_last) * P.ld_ws + at);
+        copy4(dst + 128 * SCALE_PITCH + lane, P.ws + static_cast<long long>(nb < nb_last ? nb : nb_last) * P.ld_ws + at);
     }
-    for (int j = FIRST / 4; j < (FIRST + ROWS) / 4; j += AHEAD) {
-        float x[AHEAD];
+#pragma unroll 8
+    for (int r = FIRST + (lane >> 3); r < FIRST + ROWS; r += 4) {
+        const int m = m0 + r < P.M ? m0 + r : P.M - 1;
+        copy4(dst + r * SCALE_PITCH + (lane & 7), P.xs + m * P.ld_xs + at);
+    }
+}
+
+// Starts a warp's copy of a vector's 128 values from n0 on; zero where there are none.  A vector may start anywhere.
+__device__ __forceinline__ void copy_vector(const Params& P, float* dst, const float* src, int n0, int lane) {
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const int r = 4 * (j + i) + (lane >> 3);
-            const int m = m0 + r < P.M ? m0 + r : P.M - 1;
-            x[i] = __ldg(P.xs + m * P.ld_xs + at);
-        }
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) dst[(4 * (j + i) + (lane >> 3)) * SCALE_PITCH + (lane & 7)] = x[i];
+    for (int i = 0; i < 4; ++i) {
+        const int c = 32 * i + lane;
+        const bool in = src != nullptr && n0 + c < P.N;
+        copy4(dst + c, in ? src + n0 + c : P.xs, in);
     }
 }
 
@@ -524,10 +538,11 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             if (!__all_sync(0xffffffffu, mbar_wait(&sc_empty[g & 1], ((g >> 1) & 1) ^ 1u, abort_flag, P.err))) break;
             const int at = b_first + (b + (lane & 7) < blocks ? b + (lane & 7) : blocks - 1);
             if (warp == 2) {
-                bring_scales<0, 64, 16>(P, scales + (g & 1) * SCALE_WORDS, m0, at, n_tile, 1, lane);
+                copy_scales<0, 64>(P, scales + (g & 1) * SCALE_WORDS, m0, at, n_tile, 1, lane);
             } else {
-                bring_scales<64, 64, 16>(P, scales + (g & 1) * SCALE_WORDS, m0, at, n_tile, 1, lane);
+                copy_scales<64, 64>(P, scales + (g & 1) * SCALE_WORDS, m0, at, n_tile, 1, lane);
             }
+            copies_wait();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sc_full[g & 1]);
         }
@@ -605,7 +620,9 @@ __device__ __forceinline__ void prefetch_residual(const Params& P, int m0, int n
 // 250 clocks a group for one thread, twice that per block for a common one.
 // Warp 3 brings the scales, eight blocks of the CTA's 128 rows at a time, two groups in shared memory.  The promotion
 // warps touch no global memory while they add: tcgen05.wait::ld waited for their loads, too, and a block took 1060 clocks
-// instead of 780.
+// instead of 780.  A tile's bias and gate they copy to a place of each warp's own, asynchronously, while the sums run: a
+// barrier among the warps of a half, which one place for all four would need, has no limit and would wait for good for a
+// warp whose wait has given up.
 // Signals across the pair: the peer's warp 1 passes its full barriers on to the leader's (two arrivals there: own copies,
 // peer's); acc_empty counts the promotion warps of both CTAs; the commits arrive in both.
 // Measured: 32760 x 5120 x 13824 into f16 2.4 ms (1.9 PFLOP/s), 32760 x 13824 x 5120 into the stream 2.4 ms; loads and
@@ -617,9 +634,9 @@ constexpr int A_BYTES = 128 * BK, B_HALF = 64 * BK, STAGE_BYTES = A_BYTES + 2 * 
 constexpr int WARPS = 8;
 constexpr int CPT = 128;
 constexpr int OFF_STAGE = STAGES * STAGE_BYTES;
-constexpr int OFF_VEC = OFF_STAGE + WARPS * 32 * PITCH * 4;     // [2 tiles][2 halves][bias 128, gate 128]
+constexpr int OFF_VEC = OFF_STAGE + WARPS * 32 * PITCH * 4;     // [warp][bias 128, gate 128]
 constexpr int SCALE_WORDS = 128 * SCALE_PITCH + 16;              // a group: [row][8 blocks], then ws [half][8]
-constexpr int OFF_SCALE = OFF_VEC + 2 * 2 * 256 * 4;
+constexpr int OFF_SCALE = OFF_VEC + WARPS * 256 * 4;
 constexpr int OFF_BAR = OFF_SCALE + 2 * SCALE_WORDS * 4;
 constexpr int SMEM_BYTES = OFF_BAR + 256 + 1024;
 constexpr int THREADS = 32 * (WARPS + 4);                       // registers move in groups of four warps
@@ -684,9 +701,9 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     const uint32_t tmem_base = *tmem_slot;
 
     // 168 registers a thread at launch (384 threads); the promotion warps take what the others give up:
-    // 256 x 224 + 128 x 56 = 384 x 168
+    // 256 x 232 + 128 x 40 = 384 x 168
     if (warp >= 4) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         const int quarter = warp & 3, side = (warp - 4) >> 2;
         const int row = quarter * 32 + lane;
         float* stage = reinterpret_cast<float*>(smem + OFF_STAGE) + (warp - 4) * 32 * PITCH;
@@ -694,16 +711,17 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         uint32_t sg = 0;   // group of scales, over all tiles
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + side * 256;
         const uint32_t free0 = leader_address(&acc_empty[2 * side]), free1 = leader_address(&acc_empty[2 * side + 1]);
-        uint32_t g = 0, parity = 0;
+        float* vec = reinterpret_cast<float*>(smem + OFF_VEC) + (warp - 4) * 256;
+        uint32_t g = 0;
         bool ok = true;
-        for (int t = first; ok && t < tiles; t += step, parity ^= 1u) {
+        for (int t = first; ok && t < tiles; t += step) {
             int m_tile, n_tile;
             pair_tile_at(P, t, m_tile, n_tile);
             const int m_first = m_tile * 256 + rank * 128 + quarter * 32;   // the warp's rows
             const int nc = n_tile * 256 + side * CPT;                       // the thread's columns
-            const bool n_ok = nc + row < P.N;
-            const float bias_v = (P.bias != nullptr && n_ok) ? __ldg(P.bias + nc + row) : 0.0f;
-            const float gate_v = (P.gate != nullptr && n_ok) ? __ldg(P.gate + nc + row) : 0.0f;
+            __syncwarp();                                                   // the last tile's vectors have been read
+            copy_vector(P, vec, P.bias, nc, lane);
+            copy_vector(P, vec + 128, P.gate, nc, lane);
             float sum[CPT];
 #pragma unroll
             for (int i = 0; i < CPT; ++i) sum[i] = 0.0f;
@@ -761,10 +779,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 if (!ok) break;
             }
             if (!ok) break;
-            float* vec = reinterpret_cast<float*>(smem + OFF_VEC) + (parity * 2 + side) * 256;
-            vec[row] = bias_v;
-            vec[128 + row] = gate_v;
-            named_bar_sync(1 + side, 128);
+            copies_wait();
+            __syncwarp();
             float (&acc)[CPT] = sum;
             bias_act(acc, vec, P.act);
             float amax = 0.0f;
@@ -779,7 +795,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             store_rows(P, acc, m_first, nc, lane, stage, vec + 128, amax);
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0) {
             uint32_t s = 0, ph = 0;
             bool ok = true;
@@ -848,7 +864,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     ok = __all_sync(0xffffffffu, mbar_wait(&sc_empty[sg & 1u], ((sg >> 1) & 1u) ^ 1u, abort_flag, P.err));
                     if (!ok) break;
                     const int at = b + (lane & 7) < P.kblocks ? b + (lane & 7) : P.kblocks - 1;
-                    bring_scales<0, 128, 16>(P, dst0 + (sg & 1u) * SCALE_WORDS, m0, at, 2 * n_tile, 2, lane);
+                    copy_scales<0, 128>(P, dst0 + (sg & 1u) * SCALE_WORDS, m0, at, 2 * n_tile, 2, lane);
+                    copies_wait();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sc_full[sg & 1u]);
                     if (b == 0 && P.gate != nullptr) prefetch_residual(P, m0, n_tile * 256, lane);
