@@ -1,8 +1,13 @@
-"""The e4m3 product: what its kernels wait on."""
+"""The e4m3 product: what its kernels wait on, every output of the kernel on CTA pairs against 64 bits.  Tolerances are those of
+test_fp8_block.py."""
 import os
 import re
 
+import pytest
+import torch
+
 from conftest import PKG
+from test_fp8_block import ACTS, F8, blank, blocked, fp8_operand, linear64, randn, run_linear
 
 
 # ---------------------------------------------------------------------------------------------------- waits have an end
@@ -16,3 +21,131 @@ def test_no_barrier_among_some_of_the_warps():
     among them without a limit would wait for that warp for good.  So between set-up and teardown, where every
     thread arrives, there is none; mbarrier waits have a limit."""
     assert not re.search(r"named_bar_sync|bar\.sync|barrier\.sync|barrier\.cta", gemm_source())
+
+
+# ------------------------------------------------------------------------------------------- every output of the pair kernel
+# From 37 tiles of 256 x 256 on: ragged in both directions, one to nine blocks of 128 k, and an n that is no multiple of 4.
+PAIR_SHAPES = [(600, 72, 3333), (600, 1024, 3330), (2600, 300, 1001), (515, 1100, 3607)]
+OUTS = [torch.float32, torch.float16, torch.bfloat16, "gated", "f8"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", PAIR_SHAPES)
+@pytest.mark.parametrize("out", OUTS)
+@pytest.mark.parametrize("bias", [True, False])
+def test_pair_outputs(edb, cuda, m, k, n, out, bias):
+    run_linear(edb, m, k, n, out, bias=bias, pad=16 if m % 2 else 0, seed=m + k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", sorted(ACTS))
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("out", OUTS)
+def test_pair_activations(edb, cuda, act, bias, out):
+    run_linear(edb, 700, 200, 3402, out, act=act, bias=bias, seed=7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", PAIR_SHAPES)
+def test_pair_residual_in_place(edb, cuda, m, k, n):
+    run_linear(edb, m, k, n, "gated", in_place=True, pad=16, seed=k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", ["f8", "gated", torch.bfloat16])
+def test_pair_tiles_in_chunks(edb, cuda, out):
+    """k so long that 13 of the 21 feature tiles are walked together: a second, narrower chunk."""
+    run_linear(edb, 300, 13824, 5200, out, act="gelu_tanh", seed=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(3, 200, 77), (90, 200, 130), (700, 200, 3402)])
+def test_bias_and_gate_need_no_alignment(edb, cuda, m, k, n):
+    xq, xs = fp8_operand(m, k, 1, 1)
+    wq, ws = fp8_operand(n, k, 128, 2, 0, 0.05)
+    bias, gate, res = randn(n + 1, seed=3), randn(n + 3, seed=4), blank(m, n, torch.float32, fill=2.0)
+    y = [blank(m, n, torch.float32) for _ in range(2)]
+    w = edb.Fp8Weight(wq, ws)
+    edb.mul_mat_fp8(w, xq, xs, edb.make_epilogue(y[0], bias=bias[1:], gate=gate[3:], residual=res))
+    edb.mul_mat_fp8(w, xq, xs, edb.make_epilogue(y[1], bias=bias[1:].clone(), gate=gate[3:].clone(), residual=res))
+    assert torch.equal(*y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", [torch.float32, "f8"])
+def test_pair_is_the_same_every_run_and_row_by_row(edb, cuda, out):
+    """The same bits again, and a NaN row or scale stays in its row."""
+    m, k, n = 1000, 640, 2570
+    xq, xs = fp8_operand(m, k, 1, 3)
+    w = edb.Fp8Weight(*fp8_operand(n, k, 128, 4))
+
+    def run():
+        y = torch.zeros(m, 2576, device="cuda", dtype=F8 if out == "f8" else out)[:, :n]
+        ys = torch.zeros(m, 21, device="cuda") if out == "f8" else None
+        edb.mul_mat_fp8(w, xq, xs, edb.make_epilogue(y), ys)
+        return (y.float(), ys) if out == "f8" else (y, y[:, :1].clone())
+
+    first, first_scale = run()
+    for _ in range(5):
+        again, scale = run()
+        assert torch.equal(again, first) and torch.equal(scale, first_scale)
+    rows = torch.zeros(m, dtype=torch.bool, device="cuda")
+    for bad in (0, 127, 128, 500, 999):
+        rows[bad] = True
+        if bad % 2:
+            xs[bad, 1] = float("nan")
+        else:
+            xq[bad, 5] = float("nan")
+    got, scale = run()
+    assert bool(torch.isnan(got[rows]).all())
+    assert torch.equal(got[~rows], first[~rows]) and torch.equal(scale[~rows], first_scale[~rows])
+
+
+@pytest.mark.gpu
+def test_pair_quantised_output_of_rows_not_finite(edb, cuda):
+    """An infinity in a row's activated block reaches the next product as NaN, and its neighbours keep their scale."""
+    m, k, n = 1100, 256, 2570
+    xq, xs = fp8_operand(m, k, 1, 3)
+    wq, ws = fp8_operand(n, k, 128, 4)
+    bias = torch.zeros(n, device="cuda")
+    bias[3], bias[300], bias[2569] = float("inf"), float("-inf"), float("inf")
+    y, ys = blank(m, n, F8), torch.empty(m, 21, device="cuda")
+    edb.mul_mat_fp8(edb.Fp8Weight(wq, ws), xq, xs, edb.make_epilogue(y, bias=bias), ys)
+    plain, _ = linear64(xq, xs, wq, ws, None, "none")
+    lost = torch.isinf(bias)
+    assert torch.equal(torch.isnan(y.float()), lost[None].expand(m, n))
+    plain[:, lost] = 0.0
+    top = blocked(plain, 1, torch.float64).abs().amax((1, 3))
+    assert bool(((ys.double() * 448 - top).abs() <= top * 2.0 ** -12).all())
+
+
+@pytest.mark.gpu
+def test_pair_on_two_streams_and_in_two_recordings_at_once(edb, cuda):
+    m, k, n = 1000, 1280, 2600
+    xq, xs = fp8_operand(m, k, 1, 1)
+    w = edb.Fp8Weight(*fp8_operand(n, k, 128, 2, 0, 0.05))
+    bias = randn(n, seed=5)
+    outs = [torch.empty(m, 2608, device="cuda")[:, :n] for _ in range(5)]
+    eps = [edb.make_epilogue(o, bias=bias) for o in outs]
+    edb.mul_mat_fp8(w, xq, xs, eps[4])
+    torch.cuda.synchronize()
+    streams, graphs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for i, st in enumerate(streams):
+        with torch.cuda.stream(st):
+            graphs.append(edb.Graph(lambda i=i: edb.mul_mat_fp8(w, xq, xs, eps[i])))
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                graphs[i].launch()
+                edb.mul_mat_fp8(w, xq, xs, eps[2 + i])
+    torch.cuda.synchronize()
+    edb.poll_status()
+    for o in outs[:4]:
+        assert torch.equal(o, outs[4])
+
+
+@pytest.mark.gpu
+def test_steps_of_a_quantised_output_lie_at_borders(edb, cuda):
+    """Context rows through a whole up-projection: a byte is another than 64 bits give only where the value lies within the
+    f32 sum's error of the border between the two."""
+    run_linear(edb, 154, 1536, 6144, "f8", act="gelu_tanh", seed=11)
