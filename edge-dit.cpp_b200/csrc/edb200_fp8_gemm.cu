@@ -19,6 +19,10 @@
 namespace edb {
 namespace f8g {
 
+// A warp waits as one, so that it also gives up as one: either a single lane runs the loop (copies and MMAs of the tile and
+// few-row kernels: 256 x 5120 x 5120 17.9 us, with a vote after each wait 20.6) or each wait ends in a vote (the pair kernel,
+// where the single lane was 1 to 2 % slower).
+
 constexpr int BK = 128;                       // bytes = values of a k block
 constexpr uint32_t kFmtE4M3 = 0;              // kind::f8f6f4
 constexpr int SCALE_PITCH = 9;                // words between rows of eight scales in shared memory (no conflicts)
@@ -396,7 +400,7 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;
 // Starts the copy of one group of scales: xs of 128 rows from m0 on, this lane's block `at`, as [row][8 of SCALE_PITCH], then ws of
 // `halves` weight blocks.  Four rows of eight blocks a copy; rows past the end follow the last one.  A warp brings ROWS
 // rows.  (By loads, as many under way as registers allow, a change elsewhere in the kernel that left the compiler one
-// register less put them one behind the other: 600 x 4096 x 1024 17 us instead of 12.)
+// register less put them one behind the other: 600 x 1024 x 4096 17 us instead of 12.)
 template <int FIRST, int ROWS>
 __device__ __forceinline__ void copy_scales(const Params& P, float* dst, int m0, int at, int n_block, int halves, int lane) {
     const int nb_last = (P.N - 1) >> 7;
@@ -494,29 +498,29 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 
     if (warp == 0) {
         uint32_t s = 0, ph = 0;
-        for (int b = 0; b < blocks; ++b) {
-            if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, P.err)) break;
-            if (elect_one()) {
+        if (elect_one()) {
+            for (int b = 0; b < blocks; ++b) {
+                if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, P.err)) break;
                 uint8_t* stage = smem + s * STAGE_BYTES;
                 mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
                 tma_load_2d(stage, &map_x, &full[s], (b_first + b) * BK, m0);
                 tma_load_2d(stage + A_BYTES, &map_w, &full[s], (b_first + b) * BK, n0);
-            }
-            __syncwarp();
-            if (++s == STAGES) {
-                s = 0;
-                ph ^= 1u;
+                if (++s == STAGES) {
+                    s = 0;
+                    ph ^= 1u;
+                }
             }
         }
+        __syncwarp();
     } else if (warp == 1) {
         const uint32_t idesc = make_idesc(kDFmtF32, kFmtE4M3, kFmtE4M3, 0, 0, 128, 128);
         uint32_t s = 0, ph = 0;
-        for (int b = 0; b < blocks; ++b) {
-            const uint32_t buf = b % BUFS, aph = (b / BUFS) & 1u;
-            if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
-            if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag, P.err)) break;
-            tc_fence_after_sync();
-            if (elect_one()) {
+        if (elect_one()) {
+            for (int b = 0; b < blocks; ++b) {
+                const uint32_t buf = b % BUFS, aph = (b / BUFS) & 1u;
+                if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
+                if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag, P.err)) break;
+                tc_fence_after_sync();
                 const uint32_t a_addr = smem_u32(smem + s * STAGE_BYTES), b_addr = a_addr + A_BYTES;
 #pragma unroll
                 for (int j = 0; j < BK / 32; ++j) {
@@ -525,17 +529,17 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 }
                 mma_commit(&acc_full[buf]);
                 mma_commit(&empty[s]);
-            }
-            __syncwarp();
-            if (++s == STAGES) {
-                s = 0;
-                ph ^= 1u;
+                if (++s == STAGES) {
+                    s = 0;
+                    ph ^= 1u;
+                }
             }
         }
+        __syncwarp();
     } else if (warp == 2 || warp == 3) {   // half of the rows' scales each
         for (int b = 0; b < blocks; b += 8) {
             const int g = b >> 3;
-            if (!__all_sync(0xffffffffu, mbar_wait(&sc_empty[g & 1], ((g >> 1) & 1) ^ 1u, abort_flag, P.err))) break;
+            if (!mbar_wait_warp(&sc_empty[g & 1], ((g >> 1) & 1) ^ 1u, abort_flag, P.err)) break;
             const int at = b_first + (b + (lane & 7) < blocks ? b + (lane & 7) : blocks - 1);
             if (warp == 2) {
                 copy_scales<0, 64>(P, scales + (g & 1) * SCALE_WORDS, m0, at, n_tile, 1, lane);
@@ -556,9 +560,9 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             const uint32_t buf = b % BUFS, aph = (b / BUFS) & 1u;
             const int g = b >> 3;
             bool ok = true;
-            if ((b & 7) == 0) ok = mbar_wait(&sc_full[g & 1], (g >> 1) & 1, abort_flag, P.err);
-            ok = ok && mbar_wait(&acc_full[buf], aph, abort_flag, P.err);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            if ((b & 7) == 0) ok = mbar_wait_warp(&sc_full[g & 1], (g >> 1) & 1, abort_flag, P.err);
+            ok = ok && mbar_wait_warp(&acc_full[buf], aph, abort_flag, P.err);
+            if (!ok) break;
             tc_fence_after_sync();
             uint32_t r0[32], r1[32];
             tmem_ld_32x32b_x32(taddr + buf * 128, r0);
@@ -727,9 +731,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             for (int i = 0; i < CPT; ++i) sum[i] = 0.0f;
             // One block's reading runs into the next one's: the barrier of block b + 1 is looked at and its first columns
             // are under way before block b's last products are added.
-            ok = mbar_wait(&sc_full[sg & 1u], (sg >> 1) & 1u, abort_flag, P.err) &&
-                 mbar_wait(&acc_full[2 * side + (g & 1u)], (g >> 1) & 1u, abort_flag, P.err);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = mbar_wait_warp(&sc_full[sg & 1u], (sg >> 1) & 1u, abort_flag, P.err) &&
+                 mbar_wait_warp(&acc_full[2 * side + (g & 1u)], (g >> 1) & 1u, abort_flag, P.err);
             if (!ok) break;
             const float* sc = scales + (sg & 1u) * SCALE_WORDS;
             float scale = sc[row * SCALE_PITCH] * sc[128 * SCALE_PITCH + side * 8];
@@ -752,7 +755,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     if (lane == 0) mbar_arrive(&sc_empty[sg & 1u]);
                     ++sg;
                     sc = scales + (sg & 1u) * SCALE_WORDS;
-                    if (more) ok = __all_sync(0xffffffffu, mbar_wait(&sc_full[sg & 1u], (sg >> 1) & 1u, abort_flag, P.err));
+                    if (more) ok = mbar_wait_warp(&sc_full[sg & 1u], (sg >> 1) & 1u, abort_flag, P.err);
                 }
                 const float sx = sc[row * SCALE_PITCH + ((b + 1) & 7)], sw = sc[128 * SCALE_PITCH + side * 8 + ((b + 1) & 7)];
                 tmem_wait_ld();
@@ -769,7 +772,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     promote(sum, 64, r0, s);
                     promote(sum, 96, r1, s);
                     if (more) {
-                        ok = ok && __all_sync(0xffffffffu, mbar_wait(&acc_full[2 * side + ((g + 1) & 1u)], ((g + 1) >> 1) & 1u, abort_flag, P.err));
+                        ok = ok && mbar_wait_warp(&acc_full[2 * side + ((g + 1) & 1u)], ((g + 1) >> 1) & 1u, abort_flag, P.err);
                         if (!ok) break;
                         tc_fence_after_sync();
                         tmem_ld_32x32b_x32(next, r0);
@@ -804,7 +807,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 pair_tile_at(P, t, m_tile, n_tile);
                 const int m0 = m_tile * 256 + rank * 128, n0 = n_tile * 256 + rank * 64;
                 for (int b = 0; b < P.kblocks; ++b) {
-                    if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, P.err)) {
+                    if (!mbar_wait_warp(&empty[s], ph ^ 1u, abort_flag, P.err)) {
                         ok = false;
                         break;
                     }
@@ -832,11 +835,11 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             for (int g = 0; g < blocks; ++g) {   // k blocks of all this pair's tiles
                 const uint32_t buf = g & 1u, aph = (g >> 1) & 1u;
                 // the stage first: it is there long before the accumulator, whose signal should find nothing left to wait for
-                if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
+                if (!mbar_wait_warp(&full[s], ph, abort_flag, P.err)) break;
                 const uint32_t d = tmem_base + half * 256 + buf * 128;
                 const uint32_t off = s * (STAGE_BYTES >> 4);   // descriptors count 16-byte units
                 const uint64_t a_desc = a_desc0 + off, b_desc = b_desc0 + off;
-                if (!mbar_wait(&acc_empty[2 * half + buf], aph ^ 1u, abort_flag, P.err)) break;
+                if (!mbar_wait_warp(&acc_empty[2 * half + buf], aph ^ 1u, abort_flag, P.err)) break;
                 tc_fence_after_sync();
                 if (elect_one()) {
 #pragma unroll
@@ -861,7 +864,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 pair_tile_at(P, t, m_tile, n_tile);
                 const int m0 = m_tile * 256 + rank * 128;
                 for (int b = 0; b < P.kblocks; b += 8, ++sg) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sc_empty[sg & 1u], ((sg >> 1) & 1u) ^ 1u, abort_flag, P.err));
+                    ok = mbar_wait_warp(&sc_empty[sg & 1u], ((sg >> 1) & 1u) ^ 1u, abort_flag, P.err);
                     if (!ok) break;
                     const int at = b + (lane & 7) < P.kblocks ? b + (lane & 7) : P.kblocks - 1;
                     copy_scales<0, 128>(P, dst0 + (sg & 1u) * SCALE_WORDS, m0, at, 2 * n_tile, 2, lane);
@@ -875,7 +878,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             const int blocks = first < tiles ? ((tiles - first + step - 1) / step) * P.kblocks : 0;
             uint32_t s = 0, ph = 0;
             for (int g = 0; g < blocks; ++g) {
-                if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
+                if (!mbar_wait_warp(&full[s], ph, abort_flag, P.err)) break;
                 if (elect_one()) mbar_arrive_leader(&full[s]);
                 __syncwarp();
                 if (++s == STAGES) {
@@ -977,29 +980,29 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 
     if (warp == 0) {
         uint32_t s = 0, ph = 0;
-        for (int b = 0; b < blocks; ++b) {
-            if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, P.err)) break;
-            if (elect_one()) {
+        if (elect_one()) {
+            for (int b = 0; b < blocks; ++b) {
+                if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, P.err)) break;
                 uint8_t* stage = smem + s * L::STAGE_BYTES;
                 mbar_arrive_expect_tx(&full[s], L::STAGE_BYTES);
                 tma_load_2d(stage, &map_w, &full[s], (b_first + b) * BK, n0);
                 tma_load_2d(stage + W_BYTES, &map_x, &full[s], (b_first + b) * BK, m0);
-            }
-            __syncwarp();
-            if (++s == L::STAGES) {
-                s = 0;
-                ph ^= 1u;
+                if (++s == L::STAGES) {
+                    s = 0;
+                    ph ^= 1u;
+                }
             }
         }
+        __syncwarp();
     } else if (warp == 1) {
         const uint32_t idesc = make_idesc(kDFmtF32, kFmtE4M3, kFmtE4M3, 0, 0, 128, NT);
         uint32_t s = 0, ph = 0;
-        for (int b = 0; b < blocks; ++b) {
-            const uint32_t buf = b % L::BUFS, aph = (b / L::BUFS) & 1u;
-            if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
-            if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag, P.err)) break;
-            tc_fence_after_sync();
-            if (elect_one()) {
+        if (elect_one()) {
+            for (int b = 0; b < blocks; ++b) {
+                const uint32_t buf = b % L::BUFS, aph = (b / L::BUFS) & 1u;
+                if (!mbar_wait(&full[s], ph, abort_flag, P.err)) break;
+                if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag, P.err)) break;
+                tc_fence_after_sync();
                 const uint32_t a_addr = smem_u32(smem + s * L::STAGE_BYTES), b_addr = a_addr + W_BYTES;
 #pragma unroll
                 for (int j = 0; j < BK / 32; ++j) {
@@ -1008,18 +1011,18 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
                 }
                 mma_commit(&acc_full[buf]);
                 mma_commit(&empty[s]);
-            }
-            __syncwarp();
-            if (++s == L::STAGES) {
-                s = 0;
-                ph ^= 1u;
+                if (++s == L::STAGES) {
+                    s = 0;
+                    ph ^= 1u;
+                }
             }
         }
+        __syncwarp();
     } else if (warp == 2) {
         const float* ws = P.ws + static_cast<long long>(n_tile) * P.ld_ws;
         for (int b = 0; b < blocks; b += 8) {
             const int g = b >> 3;
-            if (!__all_sync(0xffffffffu, mbar_wait(&sc_empty[g & 1], ((g >> 1) & 1) ^ 1u, abort_flag, P.err))) break;
+            if (!mbar_wait_warp(&sc_empty[g & 1], ((g >> 1) & 1) ^ 1u, abort_flag, P.err)) break;
             float* dst = scales + (g & 1) * 8 * (NT + 4) + (lane & 7) * (NT + 4) + (lane >> 3);
             const int at = b_first + (b + (lane & 7) < blocks ? b + (lane & 7) : blocks - 1);
             const float w = __ldg(ws + at);
@@ -1039,9 +1042,9 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             const uint32_t buf = b % L::BUFS, aph = (b / L::BUFS) & 1u;
             const int g = b >> 3;
             bool ok = true;
-            if ((b & 7) == 0) ok = mbar_wait(&sc_full[g & 1], (g >> 1) & 1, abort_flag, P.err);
-            ok = ok && mbar_wait(&acc_full[buf], aph, abort_flag, P.err);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            if ((b & 7) == 0) ok = mbar_wait_warp(&sc_full[g & 1], (g >> 1) & 1, abort_flag, P.err);
+            ok = ok && mbar_wait_warp(&acc_full[buf], aph, abort_flag, P.err);
+            if (!ok) break;
             tc_fence_after_sync();
             const float* sc = scales + ((g & 1) * 8 + (b & 7)) * (NT + 4);
 #pragma unroll

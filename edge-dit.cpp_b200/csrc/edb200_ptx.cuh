@@ -108,6 +108,12 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     }
 }
 
+// The same for a whole warp: one answer in all lanes.  Each lane waits for itself and may see the end of the phase or of its
+// patience by itself; a warp that leaves a loop in part would leave the rest at its next warp-wide instruction for good.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err));
+}
+
 // ------------------------------------------------------------------ fences --
 __device__ __forceinline__ void fence_proxy_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

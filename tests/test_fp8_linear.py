@@ -23,6 +23,26 @@ def test_no_barrier_among_some_of_the_warps():
     assert not re.search(r"named_bar_sync|bar\.sync|barrier\.sync|barrier\.cta", gemm_source())
 
 
+def test_a_warp_gives_up_as_one():
+    """A lane that leaves a loop alone leaves the others at elect.sync, or at a load from tensor memory, for good.  So a wait is
+    voted on by its warp, or made by one lane in a loop without any instruction for the whole warp."""
+    src, rest = gemm_source(), ""
+    blocks = []
+    while (at := src.find("if (elect_one()) {")) >= 0:
+        depth, end = 1, at + len("if (elect_one()) {")
+        while depth:
+            depth += {"{": 1, "}": -1}.get(src[end], 0)
+            end += 1
+        blocks.append(src[at + len("if (elect_one()) {"):end])
+        rest, src = rest + src[:at], src[end:]
+    rest += src
+    waits = re.compile(r"\bmbar_wait\(")
+    assert sum(len(waits.findall(b)) for b in blocks) >= 6 and "mbar_wait_warp(" in rest
+    assert not waits.search(rest)
+    for b in blocks:
+        assert not re.search(r"__syncwarp|__all_sync|__shfl|__any_sync|elect_one|mbar_wait_warp|tmem_ld|tmem_wait|__syncthreads", b)
+
+
 # ------------------------------------------------------------------------------------------- every output of the pair kernel
 # From 37 tiles of 256 x 256 on: ragged in both directions, one to nine blocks of 128 k, and an n that is no multiple of 4.
 PAIR_SHAPES = [(600, 72, 3333), (600, 1024, 3330), (2600, 300, 1001), (515, 1100, 3607)]
