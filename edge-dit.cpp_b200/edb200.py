@@ -32,6 +32,8 @@ class Epilogue(C.Structure):
         ("split_n", c_i64), ("out2", c_vp), ("out2_dtype", C.c_int), ("ldo2", c_i64), ("act2", C.c_int),
         ("split_k", C.c_int), ("pack", c_vp),
     ]
+    tensors = None      # of make_epilogue
+    fits = None         # mul_mat_fp8: rows, features and device that they have been checked for
 
 
 class QkPack(C.Structure):
@@ -400,7 +402,9 @@ class QWeight:
 
 def make_epilogue(out, bias=None, act=ACT_NONE, residual=None, gate=None, split_n=0, out2=None, act2=ACT_NONE,
                   ldo=None, ldo2=None, split_k=0):
+    """An Epilogue over torch tensors, which it keeps alive."""
     ep = Epilogue()
+    ep.tensors = {"out": out, "bias": bias, "residual": residual, "gate": gate, "out2": out2}
     ep.bias = ptr(bias)
     ep.act = act
     ep.out = ptr(out)
@@ -486,14 +490,53 @@ class Fp8Weight:
         self.ref = C.byref(self.desc)
 
 
+def _rows_inside(t, ld, m, n, what):
+    """Refuses m >= 1 rows of n values, ld apart, that t does not hold."""
+    if ld != t.stride(0):   # the caller's own stride: all that is known is where the buffer ends
+        inside = (m - 1) * ld + n <= t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+    elif t.dim() == 1:
+        inside = m == 1 and t.shape[0] >= n and t.is_contiguous()
+    else:
+        inside = t.shape[0] >= m and t[0].numel() >= n and (t[0].is_contiguous() or n == 1)
+    if not inside:
+        raise ValueError(f"mul_mat_fp8: {what} must hold {m} rows of {n} values each")
+
+
+def _check_epilogue(ep, m, n, device):
+    """The tensors of an epilogue against a product's size and place.  One whose address in `ep` was set by hand is the caller's."""
+    def kept(what):
+        t = ep.tensors[what]
+        return t if t is not None and t.data_ptr() == (getattr(ep, what) or 0) else None
+
+    out, bias, gate, residual = kept("out"), kept("bias"), kept("gate"), kept("residual")
+    for t, what in ((out, "out"), (bias, "bias"), (gate, "gate"), (residual, "residual")):
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"mul_mat_fp8: {what} is on {t.device}, the rows are on another device")
+    for t, what in ((bias, "bias"), (gate, "gate")):
+        if t is not None and (t.numel() != n or torch_dtype_id(t) != TYPE_F32 or not t.is_contiguous()):
+            raise ValueError(f"mul_mat_fp8: {what} must be contiguous float32 [{n}]")
+    if m > 0 and out is not None:
+        _rows_inside(out, ep.ldo, m, n, "out")
+    if m > 0 and residual is not None and ep.gate:   # not read without a gate
+        if torch_dtype_id(residual) != TYPE_F32:
+            raise ValueError("mul_mat_fp8: residual must be float32")
+        _rows_inside(residual, ep.ld_res, m, n, "residual")
+    ep.fits = (m, n, device)
+
+
 def mul_mat_fp8(w: Fp8Weight, x, x_scale, ep: Epilogue, out_scale=None):
     """edb200_mul_mat_fp8 on the current stream: x float8_e4m3fn [m, k], x_scale float32 [m, ceil(k / 128)], ep from
-    make_epilogue; out_scale float32 [m, ceil(n / 128)] where the epilogue's output is float8_e4m3fn."""
+    make_epilogue (bias and gate [n], out and residual [m, n]; where out has more rows or columns they are left as they are,
+    so that a kept ep serves fewer rows); out_scale float32 [m, ceil(n / 128)] where the epilogue's output is float8_e4m3fn."""
     m, k = x.shape
     if k != w.k or torch_dtype_id(x) != TYPE_F8_E4M3:
         raise ValueError(f"mul_mat_fp8: x must be float8_e4m3fn with {w.k} columns")
     ldxs = _scale_rows(x_scale, m, -(-k // 128), "mul_mat_fp8: x_scale")
     ldos = _scale_rows(out_scale, m, -(-w.n // 128), "mul_mat_fp8: out_scale") if out_scale is not None else 0
+    if ep.tensors is not None:
+        fits, device = ep.fits, x.get_device()
+        if fits is None or m > fits[0] or w.n != fits[1] or device != fits[2]:
+            _check_epilogue(ep, m, w.n, device)
     st = lib().edb200_mul_mat_fp8(w.ref, x.data_ptr(), x_scale.data_ptr(), m, _rows_of(x, "x"), ldxs, C.byref(ep),
                                   out_scale.data_ptr() if out_scale is not None else None, ldos,
                                   _launch_stream((x, x_scale, w.w, w.scale, out_scale)))

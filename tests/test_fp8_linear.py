@@ -1,7 +1,9 @@
-"""The e4m3 product: what its kernels wait on, every output of the kernel on CTA pairs against 64 bits.  Tolerances are those of
-test_fp8_block.py."""
+"""The e4m3 product: what its kernels wait on, the binding's checks of its epilogue, every output of the kernel on CTA
+pairs against 64 bits.  Tolerances are those of test_fp8_block.py."""
+import gc
 import os
 import re
+import weakref
 
 import pytest
 import torch
@@ -41,6 +43,85 @@ def test_a_warp_gives_up_as_one():
     assert not waits.search(rest)
     for b in blocks:
         assert not re.search(r"__syncwarp|__all_sync|__shfl|__any_sync|elect_one|mbar_wait_warp|tmem_ld|tmem_wait|__syncthreads", b)
+
+
+# ------------------------------------------------------------------------------------------------ epilogues that do not fit
+def product(edb, m=4, k=256, n=130, **ep):
+    """A product's arguments on the CPU, as far as the checks go; ep is built over them."""
+    z = torch.zeros
+    args = dict(w=edb.Fp8Weight(z(n, k, dtype=F8), z(-(-n // 128), 2)), x=z(m, k, dtype=F8), x_scale=z(m, 2))
+    return args, edb.make_epilogue(**{**dict(out=z(4, 144)[:, :130]), **ep})
+
+
+def test_epilogue_refusals(edb):
+    z = torch.zeros
+    gated = dict(gate=z(130), residual=z(4, 130))
+    for ep, text in (
+        (dict(out=z(3, 130)), "out must hold 4 rows"), (dict(out=z(4, 128)), "out must hold 4 rows"),
+        (dict(out=z(4, 129)), "out must hold"), (dict(out=z(130)), "out must hold"), (dict(out=z(130, 4).t()), "out must hold"),
+        (dict(out=z(3, 144), ldo=160), "out must hold"), (dict(bias=z(129)), "bias"), (dict(bias=z(131)), "bias"),
+        (dict(bias=z(130, dtype=torch.float16)), "bias"), (dict(bias=z(260)[::2]), "bias"), (dict(gated, gate=z(128)), "gate"),
+        (dict(gated, gate=z(130, dtype=torch.bfloat16)), "gate"), (dict(gated, residual=z(3, 130)), "residual must hold"),
+        (dict(gated, residual=z(4, 120)), "residual must hold"), (dict(gated, residual=z(4, 130, dtype=torch.float16)), "residual"),
+    ):
+        args, e = product(edb, **ep)
+        with pytest.raises(ValueError, match=text):
+            edb.mul_mat_fp8(ep=e, **args)
+
+
+def test_epilogue_kept_for_longer_rows_is_refused(edb):
+    """What was checked for four rows does not pass for five, nor for another weight."""
+    _, e = product(edb)
+    edb._check_epilogue(e, 4, 130, -1)
+    assert e.fits == (4, 130, -1)
+    for m, n in ((5, 130), (4, 145)):
+        args, _ = product(edb, m=m, n=n)
+        with pytest.raises(ValueError, match="out must hold"):
+            edb.mul_mat_fp8(ep=e, **args)
+
+
+def test_epilogues_that_fit(edb):
+    """A row alone, fewer rows than the buffer, a stride of the caller's, a residual that no gate asks for, addresses set by hand."""
+    z = torch.zeros
+    for m, ep in ((1, dict(out=z(130))), (4, dict(out=z(4, 144))), (2, dict(out=z(4, 130))), (4, dict(out=z(4, 2, 65))), (4, dict(out=z(4 * 144), ldo=144)),
+                  (4, dict(residual=z(2, 2, dtype=torch.float16))), (4, dict(bias=z(1, 130)))):
+        edb._check_epilogue(product(edb, **ep)[1], m, 130, -1)
+    by_hand = product(edb, out=z(1, 130))[1]
+    by_hand.out = z(9, 144).data_ptr()
+    edb._check_epilogue(by_hand, 9, 130, -1)
+    raw = edb.Epilogue()
+    assert raw.tensors is None and by_hand.tensors is not None
+
+
+def test_epilogue_keeps_its_tensors(edb):
+    bias = torch.zeros(130)
+    seen = weakref.ref(bias)
+    _, e = product(edb, bias=bias)
+    del bias
+    gc.collect()
+    assert seen() is not None and seen().data_ptr() == e.bias
+    del e, _
+    gc.collect()
+    assert seen() is None
+
+
+@pytest.mark.gpu
+def test_epilogue_places(edb, cuda):
+    """Every tensor of the epilogue on the current device; a kept epilogue serves fewer rows and leaves the others."""
+    k, n = 256, 130
+    xq, xs = fp8_operand(6, k, 1, 1)
+    w = edb.Fp8Weight(*fp8_operand(n, k, 128, 2))
+    out, res, gate, bias = blank(6, n, torch.float32), randn(6, 144)[:, :n], randn(n), randn(n)
+    good = dict(out=out, residual=res, gate=gate, bias=bias)
+    for name in good:
+        with pytest.raises(ValueError, match=f"{name} is on cpu"):
+            edb.mul_mat_fp8(w, xq, xs, edb.make_epilogue(**{**good, name: good[name].cpu()}))
+    ep = edb.make_epilogue(**good)
+    edb.mul_mat_fp8(w, xq, xs, ep)
+    whole = out.clone()
+    out.fill_(5.0)
+    edb.mul_mat_fp8(w, xq[:2], xs[:2], ep)
+    assert torch.equal(out[:2], whole[:2]) and bool((out[2:] == 5.0).all())
 
 
 # ------------------------------------------------------------------------------------------- every output of the pair kernel
