@@ -84,14 +84,35 @@ __device__ __forceinline__ void promote(float (&acc)[N], int at, const uint32_t 
     }
 }
 
-// The activations by exp and one division: gelu_tanh(v) = v / (1 + exp(-2 u)), exact to a few f32 roundings.
+// v Phi(v), Phi the normal distribution's.  For v < 0 it is exp(-v^2 / 2) h, h = erfcx(|v| / sqrt 2) / 2 = t Q(t) with
+// t = 1 / (1 + 0.305 |v|) and Q of degree 7 fitted to h / t on |v| <= 13.3, beyond which the result is 0 (weighted least squares
+// towards equal relative errors; 0.305 makes them least, 1.7 u at u = 2^-24).  The relative error stays below (24 + 1.5 v^2) u:
+// by 1 + erf, which cancels, it was 4 % at -5.  (The library's erfc in its place: 32760 x 5120 x 13824 into e4m3 4.4 ms, so 2.6.)
+__device__ __forceinline__ float gelu_erf(float v) {
+    const float t = __fdividef(1.0f, fmaf(0.305f, fabsf(v), 1.0f));
+    float q = 0.0366991907f;
+    q = fmaf(q, t, -0.1529883f);
+    q = fmaf(q, t, 0.185716853f);
+    q = fmaf(q, t, -0.0379767865f);
+    q = fmaf(q, t, 0.121021658f);
+    q = fmaf(q, t, 0.103420876f);
+    q = fmaf(q, t, 0.122466817f);
+    q = fmaf(q, t, 0.121639736f);
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * v * -0.72134752f));   // -log2(e) / 2
+    const float below = e * (q * t);
+    return v * (v < 0.0f ? below : 1.0f - below);
+}
+// The others by exp and one division: gelu_tanh(v) = v / (1 + exp(-t)).  The fast exponential is off by 2 + 1.173 |argument|
+// steps, so the relative error grows towards the negative tail: (9 + 2.4 |v|) u for SiLU, (9 + 8.4 |t|) u for gelu_tanh;
+// where the divisor passes 2^126 the result is 0.
 __device__ __forceinline__ float act_one(float v, int act) {
     if (act == EDB200_ACT_GELU_TANH) {
         const float u = 0.7978845608028654f * v * fmaf(0.044715f * v, v, 1.0f);
         return __fdividef(v, 1.0f + __expf(-2.0f * u));
     }
     if (act == EDB200_ACT_SILU) return __fdividef(v, 1.0f + __expf(-v));
-    return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));   // EDB200_ACT_GELU_ERF
+    return gelu_erf(v);
 }
 template <int N>
 __device__ __forceinline__ void bias_act(float (&v)[N], const float* bias, int act) {

@@ -49,7 +49,7 @@ enum {
 };
 
 enum { EDB200_SPLIT_K_NEVER = 0, EDB200_SPLIT_K_UNORDERED = 1 };
-enum { EDB200_ACT_NONE = 0, EDB200_ACT_GELU_TANH = 1, EDB200_ACT_SILU = 2, EDB200_ACT_GELU_ERF = 3 /* dense f32 linear only */ };
+enum { EDB200_ACT_NONE = 0, EDB200_ACT_GELU_TANH = 1, EDB200_ACT_SILU = 2, EDB200_ACT_GELU_ERF = 3 /* dense f32 and e4m3 linears */ };
 
 /* Buffers of every rank of the group as this GPU addresses them (peer mappings over
  * NVLink, see edb200_comm_map_peers): buf[i][r] = buffer i of rank r.  Kernels that

@@ -1,6 +1,7 @@
 """The e4m3 product: what its kernels wait on, the binding's checks of its epilogue, every output of the kernel on CTA
 pairs against 64 bits.  Tolerances are those of test_fp8_block.py."""
 import gc
+import math
 import os
 import re
 import weakref
@@ -9,7 +10,7 @@ import pytest
 import torch
 
 from conftest import PKG
-from test_fp8_block import ACTS, F8, blank, blocked, fp8_operand, linear64, randn, run_linear
+from test_fp8_block import ACTS, F8, U32, blank, blocked, fp8_operand, linear64, randn, run_linear
 
 
 # ---------------------------------------------------------------------------------------------------- waits have an end
@@ -250,3 +251,31 @@ def test_steps_of_a_quantised_output_lie_at_borders(edb, cuda):
     """Context rows through a whole up-projection: a byte is another than 64 bits give only where the value lies within the
     f32 sum's error of the border between the two."""
     run_linear(edb, 154, 1536, 6144, "f8", act="gelu_tanh", seed=11)
+
+
+# ------------------------------------------------------------------------------------------- activations far from zero
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 90, 700])
+@pytest.mark.parametrize("act", ["gelu_erf", "gelu_tanh", "silu"])
+def test_activations_of_negative_values_keep_their_relative_error(edb, cuda, m, act):
+    """Rows of zeros and a bias: the activation's argument is exact, and its value is compared relative to itself.
+
+    u = 2^-24, and each constant and operation rounds once unless said.  gelu_erf: -v^2 / 2 by three roundings makes
+    1.5 v^2 u of the exponential, its approximation 3 u (2^-22.5); t = 1 / (1 + 0.305 |v|) is off by 5 u (the fast division by 2
+    steps), which h turns into at most 2.62 times as much; the polynomial's sums 3.1 u, its fit 1.7 u, three products:
+    (24 + 1.5 v^2) u.  silu: __expf(x) by 2 + 1.173 |x| steps of 2 u, the sum by u, the fast division by 4 u:
+    (9 + 2.35 |v|) u.  gelu_tanh: its exponent t takes six roundings besides: (9 + 8.35 |t|) u."""
+    n = 2602
+    low, high = {"gelu_erf": (-12.0, 6.0), "gelu_tanh": (-9.0, 9.0), "silu": (-85.0, 20.0)}[act]
+    v = torch.linspace(low, high, n, device="cuda")
+    w = edb.Fp8Weight(torch.zeros(n, 128, device="cuda", dtype=F8), torch.ones(21, 1, device="cuda"))
+    y = blank(m, n, torch.float32)
+    edb.mul_mat_fp8(w, torch.zeros(m, 128, device="cuda", dtype=F8), torch.ones(m, 1, device="cuda"),
+                    edb.make_epilogue(y, bias=v, act=ACTS[act]))
+    x = v.double()
+    t = 2 * math.sqrt(2 / math.pi) * (x + 0.044715 * x ** 3)
+    want, roundings = {"gelu_erf": (0.5 * x * torch.erfc(-x / math.sqrt(2)), 24 + 1.5 * x * x),
+                       "gelu_tanh": (x * torch.sigmoid(t), 9 + 8.35 * t.abs()),
+                       "silu": (x * torch.sigmoid(x), 9 + 2.35 * x.abs())}[act]
+    off = (y.double() - want).abs() / (want.abs() * U32 * roundings * (1 + 2.0 ** -10))
+    assert bool((off[:, want != 0] <= 1).all()), off.nan_to_num().max().item()
