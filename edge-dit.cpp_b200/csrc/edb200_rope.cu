@@ -322,6 +322,9 @@ edb200_status_t edb200_rope_apply(const edb200_rope_t* r, const edb200_rope_tens
         vec = vec && ((reinterpret_cast<uintptr_t>(t.in) | reinterpret_cast<uintptr_t>(t.out)) & 15u) == 0;
         P.t[i] = {t.in, t.out, t.in_token, t.in_head, t.out_token, t.out_head, t.heads};
     }
+    if (ts[1] != nullptr && (q->out == k->out || q->out == k->in || k->out == q->in)) {
+        return fail(EDB200_ERR_INVALID, "rope_apply: one tensor's out may not be the other's out or in");
+    }
     if (reinterpret_cast<uintptr_t>(positions) & 3u) return fail(EDB200_ERR_INVALID, "rope_apply: positions must be 4-byte aligned");
     P.positions = positions;
     P.tokens = tokens;

@@ -647,6 +647,8 @@ class Rope:
             at = positions.data_ptr()
         b = None
         if k is not None:
+            if k_out is None:
+                raise ValueError("Rope: k needs k_out")
             if k.shape[0] != tokens or k.shape[2] != d or k.dtype != q.dtype:
                 raise ValueError("Rope: q and k share tokens, d_head and type")
             b = C.byref(self._tensor(k, k_out))

@@ -465,7 +465,7 @@ EDB200_API edb200_status_t edb200_rope_create(const edb200_rope_config_t* cfg, e
 EDB200_API void edb200_rope_destroy(edb200_rope_t* r);
 /* One or two tensors (q and k) of f32 / f16 / bf16, [tokens, heads, d_head] in any order: element strides between
  * tokens and between heads, channels contiguous.  Strides of out laid head-major give attention operands.  out may
- * be in itself (same strides); otherwise the two do not overlap.  positions: [tokens, n_axes] int32 on the device,
+ * be in itself (same strides); otherwise it overlaps no in, and no other out.  positions: [tokens, n_axes] int32 on the device,
  * or NULL = the token's index on every axis.  inverse turns back (the gradient of the forward call, multiplier
  * included).  k with k->in NULL or k NULL: q alone. */
 typedef struct {
