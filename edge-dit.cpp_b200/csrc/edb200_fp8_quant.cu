@@ -69,7 +69,8 @@ __device__ __forceinline__ float group_max(float a) {
 }
 
 // 1 x 128: a group of eight lanes per block.  SMALL: the block's row by the product with 2^32 / kb rounded up, exact while
-// blocks times kb stay below 2^32; else by division in 64 bits.
+// blocks times kb stay below 2^32; else by division in 64 bits, which costs nothing beside the memory (372000 x 13824 bf16
+// 2.58 ms, 365000 rows by the product 2.45).  VEC: whether rows are aligned is another matter than how many there are.
 template <typename T, bool VEC, bool SMALL>
 __global__ void __launch_bounds__(THREADS)
 quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int k, int kb, uint32_t inv_kb, uint8_t* __restrict__ q,
@@ -169,13 +170,9 @@ static edb200_status_t launch(const T* x, int64_t ldx, int64_t rows, int64_t k, 
         const int kbi = static_cast<int>(kb);
         const uint32_t inv_kb = static_cast<uint32_t>((0x100000000ull + kb - 1) / kb);
         const bool small = static_cast<double>(ctas) * (THREADS / 8) * static_cast<double>(kb) < 4294967296.0;
-        if (!small) {
-            quantize_rows_kernel<T, false, false><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, kbi, inv_kb, q, ldq, scale, ld_scale);
-        } else if (vec) {
-            quantize_rows_kernel<T, true, true><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, kbi, inv_kb, q, ldq, scale, ld_scale);
-        } else {
-            quantize_rows_kernel<T, false, true><<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, kbi, inv_kb, q, ldq, scale, ld_scale);
-        }
+        auto kernel = small ? (vec ? quantize_rows_kernel<T, true, true> : quantize_rows_kernel<T, false, true>)
+                            : (vec ? quantize_rows_kernel<T, true, false> : quantize_rows_kernel<T, false, false>);
+        kernel<<<grid, THREADS, 0, s>>>(x, ldx, rows, ki, kbi, inv_kb, q, ldq, scale, ld_scale);
     } else {
         const int64_t rb = (rows + 127) / 128;
         if (rb > 65535) return fail(EDB200_ERR_UNSUPPORTED, "quantize_fp8: more than 65535 x 128 rows of 128 x 128 blocks");
