@@ -71,6 +71,16 @@ PFN_encodeTiled get_encode_tiled() {
     return fn;
 }
 
+// The encoder is a driver call and needs a current context, which a thread has only from its first runtime call that binds one
+// on (cudaGetDevice does not): a thread of its own may come here before that.
+template <typename... A>
+static CUresult encode(PFN_encodeTiled enc, A... a) {
+    CUresult r = enc(a...);
+    int dev = 0;
+    if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = enc(a...);
+    return r;
+}
+
 edb200_status_t make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dt, int elem_bytes, const void* base,
                              uint64_t inner, uint64_t outer, uint64_t pitch_bytes, uint32_t box_inner,
                              uint32_t box_outer, CUtensorMapSwizzle swz) {
@@ -84,7 +94,7 @@ edb200_status_t make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dt, int elem_
     cuuint64_t strides[1] = {pitch_bytes};
     cuuint32_t box[2] = {box_inner, box_outer};
     cuuint32_t estr[2] = {1, 1};
-    CUresult r = enc(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+    CUresult r = encode(enc, map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(EDB200_ERR_CUDA, "cuTensorMapEncodeTiled(2d) failed: %d", (int)r);
     return EDB200_OK;
@@ -103,7 +113,7 @@ edb200_status_t make_tmap_3d(CUtensorMap* map, CUtensorMapDataType dt, int elem_
     cuuint64_t strides[2] = {pitch1_bytes, pitch2_bytes};
     cuuint32_t box[3] = {b0, b1, b2};
     cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = enc(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+    CUresult r = encode(enc, map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(EDB200_ERR_CUDA, "cuTensorMapEncodeTiled(3d) failed: %d", (int)r);
     return EDB200_OK;

@@ -4,6 +4,7 @@ import gc
 import math
 import os
 import re
+import threading
 import weakref
 
 import pytest
@@ -279,3 +280,30 @@ def test_activations_of_negative_values_keep_their_relative_error(edb, cuda, m, 
                        "silu": (x * torch.sigmoid(x), 9 + 2.35 * x.abs())}[act]
     off = (y.double() - want).abs() / (want.abs() * U32 * roundings * (1 + 2.0 ** -10))
     assert bool((off[:, want != 0] <= 1).all()), off.nan_to_num().max().item()
+
+
+# ------------------------------------------------------------------------------------------------------ threads of their own
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [8, 300, 2600])
+def test_call_from_a_thread_of_its_own(edb, cuda, m):
+    """A thread that has made no CUDA call yet has no current context: the tensor maps are made all the same."""
+    k, n = 256, 1100
+    xq, xs = fp8_operand(m, k, 1, 1)
+    w = edb.Fp8Weight(*fp8_operand(n, k, 128, 2))
+    y = [torch.zeros(m, 1104, device="cuda")[:, :n] for _ in range(2)]
+    edb.mul_mat_fp8(w, xq, xs, edb.make_epilogue(y[0]))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work():
+        try:
+            edb.mul_mat_fp8(w, xq, xs, edb.make_epilogue(y[1]))
+        except Exception as e:
+            failed.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    assert torch.equal(*y)
