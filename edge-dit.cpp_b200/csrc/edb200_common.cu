@@ -120,7 +120,8 @@ edb200_status_t make_tmap_3d(CUtensorMap* map, CUtensorMapDataType dt, int elem_
 }
 
 int sm_count() {
-    static int n = 0;
+    static std::atomic<int> count{0};
+    int n = count.load(std::memory_order_relaxed);
     if (n == 0) {
         int dev = 0;
         cudaDeviceProp p;
@@ -129,6 +130,7 @@ int sm_count() {
         } else {
             n = 148;
         }
+        count.store(n, std::memory_order_relaxed);
     }
     return n;
 }

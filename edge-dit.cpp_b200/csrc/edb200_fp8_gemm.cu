@@ -14,6 +14,7 @@
 #include "edb200_ptx.cuh"
 #include "edb200_fp8.cuh"
 
+#include <atomic>
 #include <cstring>
 
 namespace edb {
@@ -1112,14 +1113,16 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     }
 }
 
-// Sets a kernel's dynamic shared memory once per device.
+// Sets a kernel's dynamic shared memory once per device (twice where two threads make the first call at once).
+using PerDevice = std::atomic<bool>[64];
 template <typename K>
-static edb200_status_t allow_smem(K kern, int bytes, bool (&done)[64]) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    if (done[dev]) return EDB200_OK;
+static edb200_status_t allow_smem(K kern, int bytes, PerDevice& done) {
+    int dev = -1;
+    EDB_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
+    const bool counted = dev >= 0 && dev < 64;
+    if (counted && done[dev].load(std::memory_order_relaxed)) return EDB200_OK;
     EDB_TRY(check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute(mul_mat_fp8)"));
-    done[dev] = true;
+    if (counted) done[dev].store(true, std::memory_order_relaxed);
     return EDB200_OK;
 }
 
@@ -1156,7 +1159,7 @@ static edb200_status_t launch_tile(const edb200_fp8_weight_t& w, const void* x, 
     CUtensorMap map_x, map_w;
     EDB_TRY(operand_map(&map_x, x, w.k, m, ldx, 128));
     EDB_TRY(operand_map(&map_w, w.w, w.k, w.n, w.ldw, 128));
-    static bool done[64] = {false};
+    static PerDevice done = {};
     EDB_TRY(allow_smem(fp8_tile_kernel, tile::SMEM_BYTES, done));
     P.m_tiles = static_cast<int>((m + 127) / 128);
     const int64_t tiles = (int64_t)P.m_tiles * ((w.n + 127) / 128);
@@ -1170,7 +1173,7 @@ static edb200_status_t launch_few(const edb200_fp8_weight_t& w, const void* x, i
     CUtensorMap map_x, map_w;
     EDB_TRY(operand_map(&map_x, x, w.k, m, ldx, NT));
     EDB_TRY(operand_map(&map_w, w.w, w.k, w.n, w.ldw, 128));
-    static bool done[64] = {false};
+    static PerDevice done = {};
     EDB_TRY(allow_smem(fp8_few_kernel<NT>, few::Plan<NT>::SMEM_BYTES, done));
     P.m_tiles = static_cast<int>((m + NT - 1) / NT);
     const int64_t tiles = (int64_t)P.m_tiles * ((w.n + 127) / 128);
@@ -1184,9 +1187,10 @@ static edb200_status_t launch_pair(const edb200_fp8_weight_t& w, const void* x, 
     CUtensorMap map_x, map_w;
     EDB_TRY(operand_map(&map_x, x, w.k, m, ldx, 128));
     EDB_TRY(operand_map(&map_w, w.w, w.k, w.n, w.ldw, 64));
-    static bool done[64] = {false};
+    static PerDevice done = {};
     EDB_TRY(allow_smem(fp8_pair_kernel, pair::SMEM_BYTES, done));
-    static int max_pairs = 0;   // CTA pairs that can be resident at once
+    static std::atomic<int> resident{0};   // CTA pairs that can be so at once
+    int max_pairs = resident.load(std::memory_order_relaxed);
     if (max_pairs == 0) {
         cudaLaunchConfig_t cfg;
         memset(&cfg, 0, sizeof(cfg));
@@ -1199,6 +1203,7 @@ static edb200_status_t launch_pair(const edb200_fp8_weight_t& w, const void* x, 
             n = sm_count() / 2;
         }
         max_pairs = n < sm_count() / 2 ? n : sm_count() / 2;
+        resident.store(max_pairs, std::memory_order_relaxed);
     }
     P.m_tiles = static_cast<int>((m + 255) / 256);
     P.n_tiles = static_cast<int>((w.n + 255) / 256);

@@ -4,6 +4,8 @@ import gc
 import math
 import os
 import re
+import subprocess
+import sys
 import threading
 import weakref
 
@@ -45,6 +47,14 @@ def test_a_warp_gives_up_as_one():
     assert not waits.search(rest)
     for b in blocks:
         assert not re.search(r"__syncwarp|__all_sync|__shfl|__any_sync|elect_one|mbar_wait_warp|tmem_ld|tmem_wait|__syncthreads", b)
+
+
+def test_nothing_plain_is_shared_between_calls():
+    """Entry points may be called from several threads: what a function keeps between calls is atomic."""
+    for name in ("fp8_gemm", "fp8_quant", "block_norm", "rope"):
+        with open(os.path.join(PKG, "csrc", f"edb200_{name}.cu")) as fh:
+            kept = re.findall(r"^[ \t]+static (?!const\b|constexpr\b)([^=;{]*)", fh.read(), re.M)
+        assert all("atomic" in k or "PerDevice" in k for k in kept), (name, kept)
 
 
 # ------------------------------------------------------------------------------------------------ epilogues that do not fit
@@ -307,3 +317,44 @@ def test_call_from_a_thread_of_its_own(edb, cuda, m):
     torch.cuda.synchronize()
     assert not failed, failed
     assert torch.equal(*y)
+
+
+FIRST_CALLS = """
+import sys, threading
+import torch
+sys.path.insert(0, sys.argv[1])
+import conftest
+edb = conftest.load_pkg_module("edb200")
+cases = []
+for m, n in ((8, 400), (30, 400), (60, 400), (300, 400), (2600, 1100)):
+    x, w = torch.randn(m, 256, device="cuda").to(torch.float8_e4m3fn), torch.randn(n, 256, device="cuda").to(torch.float8_e4m3fn)
+    xs, ws = torch.rand(m, 2, device="cuda"), torch.rand(-(-n // 128), 2, device="cuda")
+    cases.append((edb.Fp8Weight(w, ws), x, xs, [torch.empty(m, 1104, device="cuda")[:, :n] for _ in range(4)]))
+torch.cuda.synchronize()
+start, failed = threading.Barrier(4), []
+
+def work(i):
+    try:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            start.wait()
+            for w, x, xs, y in cases:
+                edb.mul_mat_fp8(w, x, xs, edb.make_epilogue(y[i]))
+            torch.cuda.current_stream().synchronize()
+    except Exception as e:
+        failed.append(e)
+
+threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert not failed, failed
+edb.poll_status()
+assert all(torch.equal(y[0], o) and bool(torch.isfinite(o).all()) for *_, y in cases for o in y)
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_from_four_threads(edb, cuda):
+    """Each kernel's first call in a process, made by four threads on streams of their own."""
+    run = subprocess.run([sys.executable, "-c", FIRST_CALLS, os.path.dirname(os.path.abspath(__file__))], capture_output=True,
+                         text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
