@@ -448,10 +448,10 @@ __device__ __forceinline__ void copy_vector(const Params& P, float* dst, const f
 }
 
 // ------------------------------------------------------------------ one CTA per 128 tokens x 128 features
-// For products whose 256 x 256 tiles are too few for the CTA pairs below (256 x 5120 x 5120 20 us; pairs 28).  Tokens in the lanes, features in the columns of
-// four accumulators; eight promotion warps of 32 tokens x 64 features, warps 2 and 3 bringing the scales as in the pairs.  Where
-// the tiles leave SMs idle a cluster of up to eight CTAs shares one, each a run of its k blocks; sums meet in shared memory
-// and are added in the order of the parts.
+// For products whose 256 x 256 tiles are too few or too empty for the CTA pairs below (256 x 5120 x 5120 17.9 us; pairs 25).
+// Tokens in the lanes, features in the columns of four accumulators; eight promotion warps of 32 tokens x 64 features,
+// warps 2 and 3 bringing the scales as in the pairs.  Where the tiles leave SMs idle a cluster of up to eight CTAs shares
+// one, each a run of its k blocks; sums meet in shared memory and are added in the order of the parts.
 namespace tile {
 constexpr int STAGES = 5, BUFS = 4;
 constexpr int A_BYTES = 128 * BK, STAGE_BYTES = 2 * A_BYTES;
@@ -1155,7 +1155,8 @@ static edb200_status_t launch_parts(K kern, int64_t tiles, int parts, int thread
     return EDB200_OK;
 }
 
-static edb200_status_t launch_tile(const edb200_fp8_weight_t& w, const void* x, int64_t m, int64_t ldx, Params& P, cudaStream_t s) {
+static edb200_status_t launch_tile(const edb200_fp8_weight_t& w, const void* x, int64_t m, int64_t ldx, int parts, Params& P,
+                                   cudaStream_t s) {
     CUtensorMap map_x, map_w;
     EDB_TRY(operand_map(&map_x, x, w.k, m, ldx, 128));
     EDB_TRY(operand_map(&map_w, w.w, w.k, w.n, w.ldw, 128));
@@ -1163,13 +1164,12 @@ static edb200_status_t launch_tile(const edb200_fp8_weight_t& w, const void* x, 
     EDB_TRY(allow_smem(fp8_tile_kernel, tile::SMEM_BYTES, done));
     P.m_tiles = static_cast<int>((m + 127) / 128);
     const int64_t tiles = (int64_t)P.m_tiles * ((w.n + 127) / 128);
-    int parts = 1;   // of k: while every tile's cluster still gets SMs of its own, four blocks each at least
-    while (parts < 8 && tiles * parts * 2 <= sm_count() && P.kblocks >= parts * 8) parts *= 2;
     return launch_parts(fp8_tile_kernel, tiles, parts, tile::THREADS, tile::SMEM_BYTES, map_x, map_w, P, s);
 }
 
 template <int NT>
-static edb200_status_t launch_few(const edb200_fp8_weight_t& w, const void* x, int64_t m, int64_t ldx, Params& P, cudaStream_t s) {
+static edb200_status_t launch_few(const edb200_fp8_weight_t& w, const void* x, int64_t m, int64_t ldx, int parts, Params& P,
+                                  cudaStream_t s) {
     CUtensorMap map_x, map_w;
     EDB_TRY(operand_map(&map_x, x, w.k, m, ldx, NT));
     EDB_TRY(operand_map(&map_w, w.w, w.k, w.n, w.ldw, 128));
@@ -1177,34 +1177,16 @@ static edb200_status_t launch_few(const edb200_fp8_weight_t& w, const void* x, i
     EDB_TRY(allow_smem(fp8_few_kernel<NT>, few::Plan<NT>::SMEM_BYTES, done));
     P.m_tiles = static_cast<int>((m + NT - 1) / NT);
     const int64_t tiles = (int64_t)P.m_tiles * ((w.n + 127) / 128);
-    // parts of k: as many as two CTAs an SM have room for, two blocks each at least
-    int parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= 2 * sm_count() && P.kblocks >= parts * 4) parts *= 2;
     return launch_parts(fp8_few_kernel<NT>, tiles, parts, few::THREADS, few::Plan<NT>::SMEM_BYTES, map_x, map_w, P, s);
 }
 
-static edb200_status_t launch_pair(const edb200_fp8_weight_t& w, const void* x, int64_t m, int64_t ldx, Params& P, cudaStream_t s) {
+static edb200_status_t launch_pair(const edb200_fp8_weight_t& w, const void* x, int64_t m, int64_t ldx, int resident, Params& P,
+                                   cudaStream_t s) {
     CUtensorMap map_x, map_w;
     EDB_TRY(operand_map(&map_x, x, w.k, m, ldx, 128));
     EDB_TRY(operand_map(&map_w, w.w, w.k, w.n, w.ldw, 64));
     static PerDevice done = {};
     EDB_TRY(allow_smem(fp8_pair_kernel, pair::SMEM_BYTES, done));
-    static std::atomic<int> resident{0};   // CTA pairs that can be so at once
-    int max_pairs = resident.load(std::memory_order_relaxed);
-    if (max_pairs == 0) {
-        cudaLaunchConfig_t cfg;
-        memset(&cfg, 0, sizeof(cfg));
-        cfg.gridDim = dim3(static_cast<unsigned>(sm_count() & ~1), 1, 1);
-        cfg.blockDim = dim3(pair::THREADS, 1, 1);
-        cfg.dynamicSmemBytes = pair::SMEM_BYTES;
-        int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, fp8_pair_kernel, &cfg) != cudaSuccess || n <= 0) {
-            (void)cudaGetLastError();
-            n = sm_count() / 2;
-        }
-        max_pairs = n < sm_count() / 2 ? n : sm_count() / 2;
-        resident.store(max_pairs, std::memory_order_relaxed);
-    }
     P.m_tiles = static_cast<int>((m + 255) / 256);
     P.n_tiles = static_cast<int>((w.n + 255) / 256);
     // feature tiles walked together: their weights, read again for every token tile, stay within about a third of L2
@@ -1212,10 +1194,89 @@ static edb200_status_t launch_pair(const edb200_fp8_weight_t& w, const void* x, 
     P.chunk = static_cast<int>(ch < 1 ? 1 : ch < P.n_tiles ? ch : P.n_tiles);
     const int64_t tiles = (int64_t)P.m_tiles * P.n_tiles;
     if (tiles > 0x3fffffff) return fail(EDB200_ERR_UNSUPPORTED, "mul_mat_fp8: too many output tiles");
-    const unsigned grid = 2u * static_cast<unsigned>(tiles < max_pairs ? tiles : max_pairs);
+    const unsigned grid = 2u * static_cast<unsigned>(tiles < resident ? tiles : resident);
     fp8_pair_kernel<<<grid, pair::THREADS, pair::SMEM_BYTES, s>>>(map_x, map_w, P);
     count_launch();
     return check_cuda(cudaGetLastError(), "mul_mat_fp8 launch");
+}
+
+// Clusters of `parts` (1, 2, 4 or 8) CTAs, one an SM, that are resident at once: 148, 74, 33 and 15 here, fewer than SMs / parts
+// because a cluster lies within one group of SMs.
+static int clusters_resident(int parts) {
+    static std::atomic<int> known[4] = {};
+    const int i = parts == 1 ? 0 : parts == 2 ? 1 : parts == 4 ? 2 : 3;
+    int n = known[i].load(std::memory_order_relaxed);
+    if (n != 0) return n;
+    const int most = sm_count() / parts;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(most * parts));
+    cfg.blockDim = dim3(tile::THREADS);
+    cfg.dynamicSmemBytes = tile::SMEM_BYTES;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = static_cast<unsigned>(parts);
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    static PerDevice done = {};
+    if (allow_smem(fp8_tile_kernel, tile::SMEM_BYTES, done) != EDB200_OK ||
+        cudaOccupancyMaxActiveClusters(&n, fp8_tile_kernel, &cfg) != cudaSuccess || n <= 0 || n > most) {
+        (void)cudaGetLastError();
+        n = most;
+    }
+    known[i].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+// Which kernel takes a product, and into how many parts its k blocks are cut: the one whose time by the sums below is least.
+// They count waves of resident CTAs; the unit is the tile kernel's block (0.31 us), and the numbers were fitted to 890 timed
+// cases (m 1 to 640, n 256 to 30720, k 512 to 13824; activations and outputs at six sizes).  There the choice costs 0.2 % over
+// the fastest on average and 11 % at worst, at 500 drawn sizes and epilogues besides 0.7 and 14 % (a fixed 37 pairs and parts by
+// the number of SMs: 6.5 and 76 %).
+// m x k x n, us:                     few rows          tiles             pairs
+//   300 x 5120 x 5120 to f16          30.0              18.4              25.4
+//    96 x 5120 x 10240 to f16         29.7              18.3              25.6   (tiles 75 % full, pairs 37)
+//   512 x 5120 x 7168 to f16                            35.3, two waves   26.5, one wave
+//   192 x 1536 x 768 to f16           6.7 in 4 parts    7.6 in 4 parts    13.1
+//   154 x 1536 x 6144, GELU to e4m3   12.4 in 2 parts   13.7              15.7
+//     1 x 512 x 13824 to f16          4.6, in two 6.1   6.1
+enum Kernel { FEW, TILE, PAIR };
+struct Choice {
+    Kernel kernel;
+    int parts;
+};
+static Choice choose(int64_t m, int64_t n, int64_t blocks, const edb200_epilogue_t& ep) {
+    const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    const auto waves = [&](int64_t tiles, int64_t resident) { return static_cast<double>(up(tiles, resident)); };
+    const bool act = ep.act != EDB200_ACT_NONE, gated = ep.gate != nullptr;
+    const bool f8 = ep.out_dtype == EDB200_TYPE_F8_E4M3, f32 = ep.out_dtype == EDB200_TYPE_F32;
+    Choice best = {FEW, 1};
+    double least = 1e300;
+    const auto offer = [&](Kernel kernel, int parts, double time) {
+        if (time < least) {
+            least = time;
+            best = {kernel, parts};
+        }
+    };
+    const int64_t rows = m <= 16 ? 16 : m <= 32 ? 32 : 64;                // of a few-row tile
+    const int64_t few = up(m, rows) * up(n, 128), tiles = up(m, 128) * up(n, 128), pairs = up(m, 256) * up(n, 256);
+    const double u = static_cast<double>(rows) / 64.0, full = m < 128 ? static_cast<double>(m) / 128.0 : 1.0;
+    // what a tile's end takes, over f16 without activation
+    const double few_end = u * ((act ? 3.5 : 0.0) + (gated ? 6.0 : 0.0) + (f8 ? 7.0 : 0.0));
+    const double tile_end = full * (4.0 + (act ? 5.0 : 0.0) + (gated ? 7.0 : 0.0) + (f8 ? 9.0 : 0.0));
+    const double pair_end = (act ? 9.0 : 0.0) + (gated ? 14.0 : f32 ? 7.0 : 0.0);
+    for (int parts = 1; parts <= 8 && (parts == 1 || blocks >= 2 * parts); parts *= 2) {   // a part of two blocks at least
+        const int64_t one = clusters_resident(parts);                      // with one CTA an SM; the few-row kernel has two,
+        const double b = static_cast<double>(up(blocks, parts)), shared = few > one ? 1.7 : 1.0;   // each the slower
+        offer(FEW, parts, waves(few, 2 * one) * ((parts == 1 ? 12.0 : 15.0 + 0.25 * parts) + 3.0 * u + shared * (0.55 + 0.75 * u) * b + few_end / parts));
+        // up to 64 rows in one wave only: beyond it the few-row kernel's two CTAs an SM keep more of the weights under way
+        if (m > 64 || (m > 32 && tiles <= one)) {
+            offer(TILE, parts, 4.0 + waves(tiles, one) * (b + 10.0 + (parts == 1 ? 0.0 : 6.0 + 0.25 * parts) + tile_end / parts));
+        }
+    }
+    if (m > 64) offer(PAIR, 1, 14.0 + waves(pairs, clusters_resident(2)) * (1.38 * static_cast<double>(blocks) + 13.0 + pair_end));
+    return best;
 }
 
 }  // namespace f8g
@@ -1292,16 +1353,13 @@ extern "C" edb200_status_t edb200_mul_mat_fp8(const edb200_fp8_weight_t* w, cons
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof(s, PROF_GEMM, 2.0 * (double)m * (double)w->n * (double)w->k,
                    (double)w->n * (double)w->k + (double)m * (double)w->k + (double)m * (double)w->n * esz);
-    // Which kernel, by measured time (k 1536 and 5120, n 1536 to 13824):
-    //   up to 64 tokens, and where tiles of 128 tokens would be half empty (129 to 192): weight streaming.  2 x 5120 x 30720
-    //     29 us (tiles 50), 64 x 5120 x 5120 13.9 (14.6), 154 x 5120 x 5120 20.4 (22.4); 96 x 5120 x 5120 19.7 (15.5).
-    //   from 37 tiles of 256 x 256 on, half of what the GPU holds: CTA pairs.  512 x 4096 x 5120 (40 tiles) 25 us (tiles 36);
-    //     256 x 5120 x 5120 (20 tiles) 28 (22).
-    //   else tiles of 128 x 128.
-    if (m <= 16) return f8g::launch_few<16>(*w, x, m, ldx, P, s);
-    if (m <= 32) return f8g::launch_few<32>(*w, x, m, ldx, P, s);
-    const int64_t pairs = ((m + 255) / 256) * ((w->n + 255) / 256);
-    if (m <= 64 || (m > 128 && m <= 192 && pairs < 37)) return f8g::launch_few<64>(*w, x, m, ldx, P, s);
-    if (pairs >= 37) return f8g::launch_pair(*w, x, m, ldx, P, s);
-    return f8g::launch_tile(*w, x, m, ldx, P, s);
+    const f8g::Choice c = f8g::choose(m, w->n, kb, *ep);
+    switch (c.kernel) {
+        case f8g::PAIR: return f8g::launch_pair(*w, x, m, ldx, f8g::clusters_resident(2), P, s);
+        case f8g::TILE: return f8g::launch_tile(*w, x, m, ldx, c.parts, P, s);
+        default: break;
+    }
+    if (m <= 16) return f8g::launch_few<16>(*w, x, m, ldx, c.parts, P, s);
+    if (m <= 32) return f8g::launch_few<32>(*w, x, m, ldx, c.parts, P, s);
+    return f8g::launch_few<64>(*w, x, m, ldx, c.parts, P, s);
 }

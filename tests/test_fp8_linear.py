@@ -137,8 +137,10 @@ def test_epilogue_places(edb, cuda):
 
 
 # ------------------------------------------------------------------------------------------- every output of the pair kernel
-# From 37 tiles of 256 x 256 on: ragged in both directions, one to nine blocks of 128 k, and an n that is no multiple of 4.
-PAIR_SHAPES = [(600, 72, 3333), (600, 1024, 3330), (2600, 300, 1001), (515, 1100, 3607)]
+# Ragged in both directions, one to nine blocks of 128 k, n no multiple of 4.  The pairs take what would be several waves of 128 x
+# 128 tiles; the shapes of one wave (the first two and the fourth) lie just below.
+PAIR_SHAPES = [(600, 72, 3333), (600, 1024, 3330), (2600, 300, 1001), (515, 1100, 3607),
+               (1290, 72, 2891), (1290, 1024, 2890), (1283, 1100, 2895), (2600, 300, 4001)]
 OUTS = [torch.float32, torch.float16, torch.bfloat16, "gated", "f8"]
 
 
@@ -169,6 +171,24 @@ def test_pair_residual_in_place(edb, cuda, m, k, n):
 def test_pair_tiles_in_chunks(edb, cuda, out):
     """k so long that 13 of the 21 feature tiles are walked together: a second, narrower chunk."""
     run_linear(edb, 300, 13824, 5200, out, act="gelu_tanh", seed=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", ["f8", "gated", torch.bfloat16])
+def test_pair_tiles_in_chunks_of_many_rows(edb, cuda, out):
+    """The same with several token tiles for each of the features'."""
+    run_linear(edb, 1300, 13824, 5200, out, act="gelu_tanh", seed=4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", [torch.float16, "f8"])
+@pytest.mark.parametrize("m,k,n", [
+    (1, 512, 1000), (12, 700, 4300), (40, 1536, 4400), (64, 768, 9000),      # few rows: parts of three blocks and more
+    (192, 1536, 768), (129, 1792, 300), (321, 1536, 250),                    # few-row clusters beyond 64 rows
+    (129, 5120, 700), (300, 5120, 1500), (128, 5120, 2304), (150, 640, 2300),   # tiles in eight, four and two parts
+    (384, 640, 4400), (257, 1280, 10300), (96, 640, 9400), (100, 300, 13000)])  # in one; pairs that would be half empty
+def test_where_the_choice_of_kernel_changes(edb, cuda, m, k, n, out):
+    run_linear(edb, m, k, n, out, seed=m + n)
 
 
 @pytest.mark.gpu
@@ -266,7 +286,7 @@ def test_steps_of_a_quantised_output_lie_at_borders(edb, cuda):
 
 # ------------------------------------------------------------------------------------------- activations far from zero
 @pytest.mark.gpu
-@pytest.mark.parametrize("m", [3, 90, 700])
+@pytest.mark.parametrize("m", [3, 90, 700, 2900])
 @pytest.mark.parametrize("act", ["gelu_erf", "gelu_tanh", "silu"])
 def test_activations_of_negative_values_keep_their_relative_error(edb, cuda, m, act):
     """Rows of zeros and a bias: the activation's argument is exact, and its value is compared relative to itself.
@@ -326,10 +346,10 @@ sys.path.insert(0, sys.argv[1])
 import conftest
 edb = conftest.load_pkg_module("edb200")
 cases = []
-for m, n in ((8, 400), (30, 400), (60, 400), (300, 400), (2600, 1100)):
+for m, n in ((8, 400), (30, 400), (60, 400), (300, 400), (2600, 1100), (300, 9000), (5000, 4000)):
     x, w = torch.randn(m, 256, device="cuda").to(torch.float8_e4m3fn), torch.randn(n, 256, device="cuda").to(torch.float8_e4m3fn)
     xs, ws = torch.rand(m, 2, device="cuda"), torch.rand(-(-n // 128), 2, device="cuda")
-    cases.append((edb.Fp8Weight(w, ws), x, xs, [torch.empty(m, 1104, device="cuda")[:, :n] for _ in range(4)]))
+    cases.append((edb.Fp8Weight(w, ws), x, xs, [torch.empty(m, -(-n // 16) * 16, device="cuda")[:, :n] for _ in range(4)]))
 torch.cuda.synchronize()
 start, failed = threading.Barrier(4), []
 
