@@ -13,8 +13,9 @@
 // maximum is one reduction over the warp.  Four blocks a warp and 64 registers a thread keep three rows of 5120 under way on
 // an SM (308 us at the first size below; two blocks a warp, one row: 388); where there are fewer rows than that, two blocks
 // a warp finish a row sooner (1 x 5120: 3.7 against 4.0 us).
-// Measured (f32 stream): 32760 x 5120 bf16 normed on both sides into e4m3 308 us (6.0 TB/s, 0.91 of the copy rate; 329
-// where the allocator placed the operands otherwise), LayerNorm into f16 299-309 us (6.5-6.7 TB/s), 154 x 1536 3.5 us.
+// Measured (f32 stream): 32760 x 5120 bf16 normed on both sides into e4m3 307 us back to back on the same operands (6.0 TB/s,
+// 0.91 of the copy rate), 333 to 351 a call where other calls and operands come between (0.80 to 0.84); into f16 315;
+// 154 x 1536 3.4 us.  Columns no multiple of four take single accesses: 32760 x 5117 739 us, so a row's h is better padded.
 #include "edb200_internal.h"
 #include "edb200_fp8.cuh"
 

@@ -86,9 +86,10 @@ __device__ __forceinline__ void promote(float (&acc)[N], int at, const uint32_t 
 }
 
 // v Phi(v), Phi the normal distribution's.  For v < 0 it is exp(-v^2 / 2) h, h = erfcx(|v| / sqrt 2) / 2 = t Q(t) with
-// t = 1 / (1 + 0.305 |v|) and Q of degree 7 fitted to h / t on |v| <= 13.3, beyond which the result is 0 (weighted least squares
-// towards equal relative errors; 0.305 makes them least, 1.7 u at u = 2^-24).  The relative error stays below (24 + 1.5 v^2) u:
-// by 1 + erf, which cancels, it was 4 % at -5.  (The library's erfc in its place: 32760 x 5120 x 13824 into e4m3 4.4 ms, so 2.6.)
+// t = 1 / (1 + 0.305 |v|) and Q of degree 7 fitted to h / t on |v| <= 13.3, beyond which the result is 0 (weighted least
+// squares towards equal relative errors; 0.305 makes them least, 1.7 u at u = 2^-24).  The relative error stays below
+// (24 + 1.5 v^2) u: by 1 + erf, which cancels, it was 4 % at -5.  (The library's erfc in its place: 32760 x 5120 x 13824 into
+// e4m3 4.4 ms, so 2.7.)
 __device__ __forceinline__ float gelu_erf(float v) {
     const float t = __fdividef(1.0f, fmaf(0.305f, fabsf(v), 1.0f));
     float q = 0.0366991907f;
@@ -419,8 +420,8 @@ __device__ __forceinline__ void copy4(float* dst, const float* src, bool in = tr
 // Waits for this thread's; the warp's after a __syncwarp.
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Starts the copy of one group of scales: xs of 128 rows from m0 on, this lane's block `at`, as [row][8 of SCALE_PITCH], then ws of
-// `halves` weight blocks.  Four rows of eight blocks a copy; rows past the end follow the last one.  A warp brings ROWS
+// Starts the copy of one group of scales: xs of 128 rows from m0 on, this lane's block `at`, as [row][8 of SCALE_PITCH], then
+// ws of `halves` weight blocks.  Four rows of eight blocks a copy; rows past the end follow the last one.  A warp brings ROWS
 // rows.  (By loads, as many under way as registers allow, a change elsewhere in the kernel that left the compiler one
 // register less put them one behind the other: 600 x 1024 x 4096 17 us instead of 12.)
 template <int FIRST, int ROWS>
@@ -651,9 +652,13 @@ __device__ __forceinline__ void prefetch_residual(const Params& P, int m0, int n
 // warp whose wait has given up.
 // Signals across the pair: the peer's warp 1 passes its full barriers on to the leader's (two arrivals there: own copies,
 // peer's); acc_empty counts the promotion warps of both CTAs; the commits arrive in both.
-// Measured: 32760 x 5120 x 13824 into f16 2.4 ms (1.9 PFLOP/s), 32760 x 13824 x 5120 into the stream 2.4 ms; loads and
-// MMAs alone 1.46 ms, MMAs alone 1.17.  Bound by the loop MMA - commit - reading - signal - MMA: two blocks an accumulator
-// pair take about 1900 clocks, of which 512 are MMAs of the half, 550 the reading, and the signals between the SMs the rest.
+// Measured, m x k x n, first launches on a rested GPU (1.9 GHz) and back to back under its power cap (1.4 to 1.6 GHz):
+//   32760 x 5120 x 13824 into f16         2.22 ms (2.1 PFLOP/s)    2.56 ms (1.8)
+//   the same, GELU into e4m3              2.33                     2.69
+//   32760 x 13824 x 5120 into the stream  2.38                     2.79
+// loads and MMAs alone 1.46 ms, MMAs alone 1.17.  Bound by the loop MMA - commit - reading - signal - MMA: two blocks an
+// accumulator pair take about 1900 clocks, of which 512 are MMAs of the half, 550 the reading (four warps of 32 lanes, each all
+// 128 columns), and the signals between the SMs the rest.  20 bytes a thread are spilled, 60 read back.
 namespace pair {
 constexpr int STAGES = 5;
 constexpr int A_BYTES = 128 * BK, B_HALF = 64 * BK, STAGE_BYTES = A_BYTES + 2 * B_HALF;
@@ -924,11 +929,12 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 }
 
 // ----------------------------------------------------------- few rows: 128 features x NT tokens, k split over a cluster
-// Bound: HBM, the weights read once (2 x 5120 x 30720 29 us, 5.4 TB/s, 0.83 of the copy rate).  The roles are turned round: features lie in the 128 lanes of tensor memory, tokens in
-// its columns, so that a tile wastes nothing on tokens that are not there; a column's scale is then one number per token
-// and block, laid out by warp 2 for eight blocks at a time.  Two CTAs share an SM and keep 160 KB of weights under way
-// there.  Where the tiles alone leave SMs idle, a cluster of up to eight CTAs takes a tile, each a run of its k blocks; the
-// partial sums meet in shared memory and are added in the order of the parts.
+// Bound: HBM, the weights read once (2 x 5120 x 30720 27.5 us, 5.7 TB/s, 0.87 of the copy rate).  The roles are turned round:
+// features lie in the 128 lanes of tensor memory, tokens in its columns, so that a tile wastes nothing on tokens that are not
+// there; a column's scale is then one number per token and block, laid out by warp 2 for eight blocks at a time.  Two CTAs
+// share an SM and keep 160 KB of weights under way there.  Where the tiles alone leave SMs idle, a cluster of up to eight
+// CTAs takes a tile, each a run of its k blocks; the partial sums meet in shared memory and are added in the order of the
+// parts.
 namespace few {
 constexpr int THREADS = 256;                 // warp 0 TMA, 1 MMA, 2 scales, 4-7 promotion; all add up and store
 constexpr int W_BYTES = 128 * BK;
@@ -1230,7 +1236,7 @@ static int clusters_resident(int parts) {
 }
 
 // Which kernel takes a product, and into how many parts its k blocks are cut: the one whose time by the sums below is least.
-// They count waves of resident CTAs; the unit is the tile kernel's block (0.31 us), and the numbers were fitted to 890 timed
+// They count waves of resident CTAs; the unit is the tile kernel's block (0.31 us), and the numbers were fitted to 878 timed
 // cases (m 1 to 640, n 256 to 30720, k 512 to 13824; activations and outputs at six sizes).  There the choice costs 0.2 % over
 // the fastest on average and 11 % at worst, at 500 drawn sizes and epilogues besides 0.7 and 14 % (a fixed 37 pairs and parts by
 // the number of SMs: 6.5 and 76 %).

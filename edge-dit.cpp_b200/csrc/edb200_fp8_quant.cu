@@ -7,7 +7,8 @@
 // 16-bit values is four full 128-byte lines and the block maximum is three shuffles.  What else bounded it was the number of
 // instructions a value: with a test for infinities on each (now on a block's maximum) 16-bit rows ran at 4.1 TB/s.
 // Measured: 32760 x 5120 bf16 rows 84 us (6.0 TB/s, 0.91 of the copy rate), 13824 x 5120 f32 in 128 x 128 blocks 53 us
-// (6.7 TB/s), the same from bf16 51 us (4.2 TB/s: a CTA loads, reduces and stores in turn, three to an SM).
+// (6.7 TB/s), the same from bf16 or f16 51 us (4.2 TB/s, floor 32: a CTA loads, reduces and stores in turn, three to an SM, and
+// values count there, not bytes).
 #include "edb200_internal.h"
 #include "edb200_fp8.cuh"
 

@@ -8,7 +8,8 @@
 // 32-bit position and below f32 rounding for positions under 10^8.  A CTA makes the cosines and sines of its few
 // tokens once, in shared memory, for all heads of q and k; then every thread turns 16-byte pieces.  Two pieces of a thread
 // under way at once cost registers and were slower (275 against 210 us).
-// Measured: 32760 tokens x 80 heads x 128 bf16 in halves 210 us (6.4 TB/s, 0.97 of the copy rate), neighbours 239 us (5.6);
+// Measured: 32760 tokens x 80 heads x 128 bf16 in halves 210 to 219 us (6.1 to 6.4 TB/s, 0.93 to 0.97 of the copy rate),
+// neighbours 239 to 242 us (5.6);
 // 154 tokens x 48 heads x 64 3.6 us.
 #include "edb200_internal.h"
 #include "edb200_fp8.cuh"

@@ -379,7 +379,7 @@ typedef struct {
 /* y[m, n] = sum over blocks b of 128 k:  x_scale[m, b] * w.scale[n / 128, b] * (sum over the block of x * w)
  * (+ bias), then the epilogue's activation and output.  x: [m, ldx] e4m3 bytes, rows on 16-byte boundaries;
  * x_scale [m, ld_xs] f32.  The products of a block are summed by the tensor cores in f32, the blocks in f32
- * registers.  Every output is one sum in one order fixed by the sizes: the same bits every run.
+ * registers.  Every output is one sum in one order fixed by the sizes and the epilogue: the same bits every run.
  * The epilogue is that of edb200_mul_mat_q (bias, act with EDB200_ACT_GELU_ERF too, gated residual with f32 out,
  * f32 / f16 / bf16 out) with these differences: bias and gate need no alignment; out_dtype may be
  * EDB200_TYPE_F8_E4M3: each row's activated columns are then quantised as edb200_quantize_fp8 does with
